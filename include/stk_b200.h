@@ -36,6 +36,7 @@ extern "C" {
 #define STK_F16 0
 #define STK_BF16 1
 #define STK_F8E4M3 2   /* sdd / dsd / dds: 8-bit float operands (1 byte each), bf16 output; see below */
+#define STK_F32 3      /* the router's gate and the token rows (top_k_gate, sort_rows, sum_rows, unsort_backward) only */
 
 /* epilogue of stk_b200_sdd */
 #define STK_EPILOGUE_NONE 0
@@ -384,6 +385,59 @@ int stk_b200_ep_dispatch(const void* x, const int32_t* order, const int32_t* off
                          int64_t row_bytes, int64_t cap_rows, void* stream);
 int stk_b200_ep_return(const void* result, const int64_t* tags, const uint64_t* peer_slots, int64_t row0,
                        int64_t n_rows, int world, int64_t row_bytes, int64_t slot_cap, void* stream);
+
+/*
+ * The router's gate, tokens sorted by expert and back with their gradients, and the experts' products
+ * from 4-bit weights (what stands around the products of a dMoE layer in training and in decoding; no
+ * counterpart in the reference).  slot = token * top_k + choice.
+ *
+ * top_k_gate: the top_k largest of every token's logits [tokens, experts] (row stride ld, element type
+ *   dtype: STK_F16 / STK_BF16 / STK_F32) and the weights of those experts, in 32 bits.  score: 0 softmax,
+ *   1 sigmoid; normalize: the weights of a token add up to 1.  Equal logits go to the lower expert; -inf is
+ *   never chosen; a choice that is left without an expert, and every choice of a token whose token_mask
+ *   byte is 0 (token_mask may be NULL), is id -1 with weight 0.  stats (float [tokens, 2]): written for the
+ *   backward pass of the plain softmax; may be NULL otherwise.  experts <= 1024, top_k <= 32.
+ * top_k_gate_backward: dlogits [tokens, experts] (contiguous) of dweights [tokens, top_k].
+ * place_tokens: stable placement of the slots in bins padded to a multiple of `block` rows.  ids[slot] =
+ *   expert, negative: none (a value >= experts counts as none and records STK_ERR_BAD_DIMS).  position[slot]
+ *   = row or -1; index[row] = slot or -1, all `rows` of it; bin_rows[e] = rows of the bin / block.  rows: a
+ *   multiple of block and at least (slots + min(slots, experts) * (block - 1)) rounded down to one, so that
+ *   every slot fits whatever the choices are.  fixed: the last expert's bin extends to `rows`.  total
+ *   (optional; may be pinned host memory): rows in use.  experts <= 1024.
+ * sort_rows: rows[r] = x[index[r] / top_k], zeros in padding (x: [tokens, hidden], row stride ld).
+ * sum_rows: out[t] = sum_j weights[t*top_k+j] * rows[position[t*top_k+j]] (weights NULL: ones), 32-bit
+ *   sums rounded once: the way back, and without weights the gradient of sort_rows.
+ * unsort_backward: the gradients of the weighted sum_rows: drows [n_rows, hidden] (zeros in padding) and
+ *   dweights [tokens, top_k]; either may be NULL.  Rows are of any length and 16-bit or 32-bit floats.
+ * int4_matvec: out[slot] = W_e x[slot / x_div] for e = ids[slot], W = (code - zero) * scale; zeros for slots
+ *   without an expert.  words / scales / zeros: as laid out by stk_b200.dmoe.pack_int4 (see
+ *   int4_sm100.cuh); zeros NULL: 8 everywhere.  dtype: of x and scales; out: the same type or, with
+ *   out_f32, float.  gelu: the exact GeLU of the product.  group 32, 64 or 128.
+ * int4_combine: out[t] = sum_j weights[slot] * y[slot] over the slots of token t that have an expert.
+ */
+int stk_b200_top_k_gate(const void* logits, int64_t ld, int64_t tokens, int experts, int top_k, int score,
+                        int normalize, const uint8_t* token_mask, float* weights, int32_t* ids, float* stats,
+                        int dtype, void* stream);
+int stk_b200_top_k_gate_backward(const void* logits, int64_t ld, int64_t tokens, int experts, int top_k, int score,
+                                 int normalize, const float* weights, const int32_t* ids, const float* stats,
+                                 const float* dweights, void* dlogits, int dtype, void* stream);
+size_t stk_b200_place_workspace_bytes(int64_t slots, int experts);
+int stk_b200_place_tokens(const int32_t* ids, int64_t slots, int experts, int block, int64_t rows, int fixed,
+                          int32_t* index, int32_t* position, int32_t* bin_rows, int64_t* total, void* workspace,
+                          size_t workspace_bytes, void* stream);
+int stk_b200_sort_rows(const void* x, int64_t ld, void* rows, const int32_t* index, const int32_t* position,
+                       int64_t tokens, int top_k, int64_t n_rows, int64_t hidden, int dtype, void* stream);
+int stk_b200_sum_rows(const void* rows, int64_t ld, const int32_t* position, const float* weights, void* out,
+                      int64_t tokens, int top_k, int64_t hidden, int dtype, void* stream);
+int stk_b200_unsort_backward(const void* dout, int64_t ld_dout, const void* rows, int64_t ld_rows,
+                             const float* weights, const int32_t* index, const int32_t* position, void* drows,
+                             float* dweights, int64_t tokens, int top_k, int64_t n_rows, int64_t hidden, int dtype,
+                             void* stream);
+int stk_b200_int4_matvec(const void* words, const void* scales, const uint8_t* zeros, const void* x,
+                         const int32_t* ids, void* out, int64_t slots, int x_div, int experts, int64_t outputs,
+                         int64_t inputs, int group, int gelu, int out_f32, int dtype, void* stream);
+int stk_b200_int4_combine(const float* y, const int32_t* ids, const float* weights, void* out, int64_t tokens,
+                          int top_k, int experts, int64_t outputs, int dtype, void* stream);
 
 /*
  * 32-bit block indices.  The reference stores block row / column indices as int16 and rejects matrices

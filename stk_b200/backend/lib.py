@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_PKG, "libstk_b200.so")
 STK_F16 = 0
 STK_BF16 = 1
 STK_F8E4M3 = 2
+STK_F32 = 3
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
@@ -68,6 +69,21 @@ SIGNATURES = {
                                           _c_i64, _c_ptr]),
     "stk_b200_ep_dispatch": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int,
                                       _c_int, _c_int, _c_int, _c_int, _c_i64, _c_i64, _c_ptr]),
+    "stk_b200_top_k_gate": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr,
+                                     _c_ptr, _c_int, _c_ptr]),
+    "stk_b200_top_k_gate_backward": (_c_int, [_c_ptr, _c_i64, _c_i64, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_ptr,
+                                              _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr]),
+    "stk_b200_place_workspace_bytes": (_c_size, [_c_i64, _c_int]),
+    "stk_b200_place_tokens": (_c_int, [_c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                       _c_ptr, _c_size, _c_ptr]),
+    "stk_b200_sort_rows": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_i64, _c_i64, _c_int,
+                                    _c_ptr]),
+    "stk_b200_sum_rows": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_i64, _c_int, _c_ptr]),
+    "stk_b200_unsort_backward": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                                          _c_i64, _c_int, _c_i64, _c_i64, _c_int, _c_ptr]),
+    "stk_b200_int4_matvec": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64,
+                                      _c_i64, _c_int, _c_int, _c_int, _c_int, _c_ptr]),
+    "stk_b200_int4_combine": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_ptr]),
     "stk_b200_ep_return": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_ptr]),
 }
 # every routine that takes or produces int16 block indices has an _i32 twin with the same signature
@@ -206,3 +222,12 @@ def dtype_code(dtype):
     if dtype == torch.float8_e4m3fn:
         return STK_F8E4M3
     raise ValueError(f"stk_b200 matmuls support float16, bfloat16 and float8_e4m3fn operands, got {dtype}")
+
+
+def row_dtype_code(dtype):
+    """Element types of the gate's logits and of token rows: those of the matmuls' 16-bit operands, and float32."""
+    if dtype == torch.float32:
+        return STK_F32
+    if dtype in (torch.float16, torch.bfloat16):
+        return dtype_code(dtype)
+    raise ValueError(f"expected float16, bfloat16 or float32, got {dtype}")

@@ -9,6 +9,9 @@
 #include "meta_sm100.cuh"
 #include "plan_sm100.cuh"
 #include "dmoe_sm100.cuh"
+#include "gate_sm100.cuh"
+#include "tokens_sm100.cuh"
+#include "int4_sm100.cuh"
 
 extern "C" int stk_b200_version(void) { return STK_B200_VERSION; }
 

@@ -18,7 +18,9 @@ import torch.distributed as dist
 
 from stk_b200.backend import kernels as _kernels
 from stk_b200.backend import lib as _lib
+from stk_b200.int4 import Int4Experts, expert_mlp_int4, int4_matvec, pack_int4, quantize_int4  # noqa: F401
 from stk_b200.matrix import Matrix
+from stk_b200.routing import TokenPlan, plan_rows, plan_tokens, sort_tokens, top_k_gate, unsort_tokens  # noqa: F401
 
 BLOCK = 128
 

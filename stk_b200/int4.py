@@ -1,0 +1,195 @@
+"""Experts with 4-bit weights for decoding: few tokens, whose products are bound by the bytes of the chosen experts'
+weights.  Public as stk_b200.dmoe.pack_int4 / quantize_int4 / int4_matvec / expert_mlp_int4.
+
+A weight stands for (code - zero) * scale, code 0..15, with a scale and a zero point (8 unless given) for each output
+row and group of 32, 64 or 128 inputs.  Beside dmoe.expert_mlp, which wants the tokens in bins of 128 rows, the
+products here take tokens and expert choices as they are.  Forward only; CUDA only, like the block-sparse products.
+The reference has no counterpart.
+"""
+import torch
+
+from stk_b200.backend import lib as _lib
+
+GROUPS = (32, 64, 128)
+
+
+class Int4Experts:
+    """The 4-bit weights [num_experts, outputs, inputs] of a set of experts in the kernels' layout (pack_int4)."""
+
+    __slots__ = ("words", "scales", "zeros", "num_experts", "outputs", "inputs", "group", "dtype")
+
+    def __init__(self, words, scales, zeros, num_experts, outputs, inputs, group):
+        self.words, self.scales, self.zeros, self.dtype = words, scales, zeros, scales.dtype
+        self.num_experts, self.outputs, self.inputs, self.group = num_experts, outputs, inputs, group
+
+    @property
+    def device(self):
+        return self.words.device
+
+    def to(self, device):
+        move = lambda t: None if t is None else t.to(device)
+        return Int4Experts(move(self.words), move(self.scales), move(self.zeros), self.num_experts, self.outputs,
+                           self.inputs, self.group)
+
+    def dequantize(self, dtype=torch.float32):
+        """The weights as numbers, [num_experts, outputs, inputs]."""
+        e, strips, chunks = self.words.shape[:3]
+        b = self.words.view(e, strips, chunks, 8, 4, 2, 2, 2, 2)                  # g, t, h, s, b, p
+        codes = torch.stack((b & 15, b >> 4), dim=-1)                             # ..., r
+        codes = codes.permute(0, 1, 9, 3, 2, 5, 4, 6, 8, 7)                       # strip r g, chunk h t s p b
+        codes = codes.reshape(e, strips * 16, chunks * 64)[:, :self.outputs, :self.inputs].to(dtype)
+        per_row = lambda t: t.transpose(2, 3).reshape(e, strips * 16, -1)[:, :self.outputs].to(dtype)
+        zero = 8 if self.zeros is None else per_row(self.zeros)[..., None]
+        codes = codes.reshape(e, self.outputs, -1, self.group) - zero
+        return (codes * per_row(self.scales)[..., None]).reshape(e, self.outputs, self.inputs)
+
+
+def pack_int4(codes, scales, zeros=None):
+    """Int4Experts from weights as checkpoints hold them.
+
+    codes: uint8 [E, N, K / 2], two codes a byte along the inputs, the lower four bits first; scales: [E, N, K / group]
+    float16 or bfloat16 (the type of the activations); zeros: uint8 [E, N, K / group] with values 0..15, or None for 8
+    everywhere.  One matrix without experts is E = 1.  Done once, when weights are loaded."""
+    if codes.dim() != 3 or codes.dtype != torch.uint8:
+        raise ValueError(f"pack_int4: codes must be uint8 [experts, outputs, inputs / 2], got {codes.dtype} "
+                         f"{tuple(codes.shape)}")
+    experts, outputs, inputs = codes.shape[0], codes.shape[1], 2 * codes.shape[2]
+    if min(experts, outputs, inputs) < 1:
+        raise ValueError(f"pack_int4: empty weights {tuple(codes.shape)}")
+    if scales.dim() != 3 or tuple(scales.shape[:2]) != (experts, outputs) or scales.shape[2] < 1 \
+            or inputs % scales.shape[2] or inputs // scales.shape[2] not in GROUPS:
+        raise ValueError(f"pack_int4: scales must be [{experts}, {outputs}, {inputs} / group] with a group of "
+                         f"{', '.join(map(str, GROUPS))} inputs, got {tuple(scales.shape)}")
+    if scales.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"pack_int4: scales are float16 or bfloat16, got {scales.dtype}")
+    if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
+        raise ValueError(f"pack_int4: zeros must be uint8 {tuple(scales.shape)}, got {zeros.dtype} {tuple(zeros.shape)}")
+    if len({t.device for t in (codes, scales, zeros) if t is not None}) > 1:
+        raise ValueError("pack_int4: codes, scales and zeros must be on one device")
+    if zeros is not None and bool((zeros > 15).any()):
+        raise ValueError("pack_int4: zero points are 0..15")
+    group, strips, chunks = inputs // scales.shape[2], (outputs + 15) // 16, (inputs + 63) // 64
+    pad = (0, 32 * chunks - inputs // 2, 0, 16 * strips - outputs)
+    words = torch.empty((experts, strips, chunks, 32, 16), dtype=torch.uint8, device=codes.device)
+    for e in range(experts):                           # (one at a time: no second copy of all weights)
+        v = torch.nn.functional.pad(codes[e], pad).view(strips, 2, 8, chunks, 2, 4, 2, 2)  # r, g, chunk, h, t, s, p
+        lo, hi = v[:, 0], v[:, 1]                      # rows g and g + 8
+        b = torch.stack(((lo & 15) | (hi << 4), (lo >> 4) | (hi & 0xF0)), dim=-2)          # ..., s, b, p
+        words[e] = b.permute(0, 2, 1, 4, 3, 5, 6, 7).reshape(strips, chunks, 32, 16)       # chunk, g, t, h, s, b, p
+    by_strip = lambda t: torch.nn.functional.pad(t, (0, 0, 0, 16 * strips - outputs)).view(
+        experts, strips, 16, -1).transpose(2, 3).contiguous()
+    return Int4Experts(words, by_strip(scales), None if zeros is None else by_strip(zeros), experts, outputs, inputs, group)
+
+
+def quantize_int4(w, group=128, zero_points=False):
+    """Int4Experts nearest to the float16 or bfloat16 weights w [E, K, N] (any strides): expert e computes x @ w[e].
+    dmoe.expert_mlp's w1 [h, E * f] is w1.view(h, E, f).transpose(0, 1), its w2 [E * f, h] is w2.view(E, f, h).
+
+    Without zero points a group's scale is its largest magnitude / 7 (codes 1..15); with them, its codes span the range
+    of the group's values and 0.  Done once, when weights are loaded."""
+    if w.dim() != 3 or w.dtype not in (torch.float16, torch.bfloat16):
+        raise ValueError(f"quantize_int4: expected float16 or bfloat16 [experts, inputs, outputs], got {w.dtype} "
+                         f"{tuple(w.shape)}")
+    if group not in GROUPS or w.shape[1] % group or w.numel() == 0:
+        raise ValueError(f"quantize_int4: the inputs must be whole groups of {', '.join(map(str, GROUPS))}, got "
+                         f"{w.shape[1]} inputs, group {group}")
+    experts, inputs, outputs = w.shape
+    codes, scales, zeros = [], [], []
+    for e in range(experts):                           # (one at a time: 32-bit copies of one expert only)
+        v = w[e].t().reshape(outputs, inputs // group, group).float()
+        if zero_points:
+            low, high = v.amin(2).clamp(max=0), v.amax(2).clamp(min=0)
+            scale = ((high - low) / 15).to(w.dtype)
+        else:
+            scale = (v.abs().amax(2) / 7).to(w.dtype)
+        # (a group of zeros, or one below the type's smallest number, keeps scale 0 and stands for zeros)
+        step = torch.where(scale > 0, scale.float(), torch.ones_like(scale, dtype=torch.float32))
+        zero = torch.round(-low / step).clamp(0, 15) if zero_points else torch.full_like(step, 8)
+        q = (torch.round(v / step[..., None]) + zero[..., None]).clamp(0, 15).to(torch.uint8).view(outputs, inputs)
+        codes.append(q[:, 0::2] | (q[:, 1::2] << 4))
+        scales.append(scale)
+        zeros.append(zero.to(torch.uint8))
+    return pack_int4(torch.stack(codes), torch.stack(scales), torch.stack(zeros) if zero_points else None)
+
+
+def _check_call(what, x, w, expert_ids):
+    if not isinstance(w, Int4Experts):
+        raise ValueError(f"{what}: weights come from pack_int4 or quantize_int4, got {type(w).__name__}")
+    if x.dim() != 2 or x.shape[1] != w.inputs:
+        raise ValueError(f"{what}: x must be [tokens, {w.inputs}], got {tuple(x.shape)}")
+    if x.dtype != w.dtype:
+        raise ValueError(f"{what}: x is {x.dtype}, the weights' scales are {w.dtype}")
+    if expert_ids is not None and (expert_ids.dim() != 2 or expert_ids.shape[0] != x.shape[0] or
+                                   expert_ids.shape[1] < 1 or
+                                   expert_ids.dtype not in (torch.int16, torch.int32, torch.int64)):
+        raise ValueError(f"{what}: expert_ids must be integers [{x.shape[0]}, k], got {expert_ids.dtype} "
+                         f"{tuple(expert_ids.shape)}")
+    if not x.is_cuda:
+        raise RuntimeError(f"{what} runs on CUDA tensors only (there is no CPU path); got a tensor on {x.device}")
+    if w.device != x.device or (expert_ids is not None and expert_ids.device != x.device):
+        raise ValueError(f"{what}: all tensors must be on one device")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError(f"{what} is forward only: x requires a gradient (call it under torch.no_grad())")
+
+
+def _matvec(x, w, ids, x_div, gelu, out):
+    with _lib.on_device(x.device):
+        rc = _lib.load().stk_b200_int4_matvec(
+            _lib.ptr(w.words), _lib.ptr(w.scales), _lib.ptr(w.zeros), _lib.ptr(x), _lib.ptr(ids), _lib.ptr(out),
+            ids.numel(), x_div, w.num_experts, w.outputs, w.inputs, w.group, int(gelu),
+            int(out.dtype == torch.float32), _lib.dtype_code(w.dtype), _lib.stream_ptr(x.device))
+    _lib.check(rc, "stk_b200_int4_matvec")
+    return out
+
+
+def _operand(x):
+    x = x.contiguous()
+    return x if x.data_ptr() % 16 == 0 else x.clone()
+
+
+def int4_matvec(x, w, expert_ids=None, gelu=False):
+    """y[t, j] = W_e x[t] for e = expert_ids[t, j]: [T, k, N] in x's type (sums in 32 bits, rounded once), zeros where
+    the id is negative; without expert_ids (weights of one expert) [T, N].  gelu: the exact GeLU of the products.
+    x [T, K] float16 or bfloat16, the type of the weights' scales.  Made for few tokens: an expert's weights are read
+    once for every 8 or 16 slots that chose it."""
+    _check_call("int4_matvec", x, w, expert_ids)
+    if expert_ids is None and w.num_experts != 1:
+        raise ValueError(f"int4_matvec: {w.num_experts} experts need expert_ids")
+    tokens = x.shape[0]
+    ids = (torch.zeros((tokens, 1), dtype=torch.int32, device=x.device) if expert_ids is None
+           else expert_ids.to(torch.int32).contiguous())
+    out = torch.empty((tokens, ids.shape[1], w.outputs), dtype=x.dtype, device=x.device)
+    _matvec(_operand(x), w, ids, ids.shape[1], gelu, out)
+    return out[:, 0] if expert_ids is None else out
+
+
+def expert_mlp_int4(x, expert_ids, weights, w1, w2):
+    """The experts' MLP of a dMoE layer on few tokens (decoding), from 4-bit weights:
+    out[t] = sum_j weights[t, j] * W2_e GeLU(W1_e x[t]), e = expert_ids[t, j], [T, h_out] in x's type.
+
+    x [T, h] float16 or bfloat16; expert_ids [T, k] and weights [T, k] as top_k_gate gives them (a negative id
+    contributes nothing); w1, w2: Int4Experts with f outputs and f inputs.  The hidden activations are rounded to x's
+    type, as in dmoe.expert_mlp; the sums over inputs and over choices are in 32 bits and rounded once."""
+    _check_call("expert_mlp_int4", x, w1, expert_ids)
+    if not isinstance(w2, Int4Experts) or w2.num_experts != w1.num_experts or w2.inputs != w1.outputs \
+            or w2.dtype != w1.dtype or w2.device != w1.device:
+        raise ValueError("expert_mlp_int4: w2 must hold the same experts, in the same type and on the same device, with "
+                         f"{w1.outputs} inputs")
+    if tuple(weights.shape) != tuple(expert_ids.shape) or weights.device != x.device:
+        raise ValueError(f"expert_mlp_int4: weights must be {tuple(expert_ids.shape)} on {x.device}, got "
+                         f"{tuple(weights.shape)} on {weights.device}")
+    _lib.row_dtype_code(weights.dtype)
+    if torch.is_grad_enabled() and weights.requires_grad:
+        raise ValueError("expert_mlp_int4 is forward only: weights require a gradient (call it under torch.no_grad())")
+    tokens, top_k = expert_ids.shape
+    dev = x.device
+    ids, weights = expert_ids.to(torch.int32).contiguous(), weights.float().contiguous()
+    hidden = _matvec(_operand(x), w1, ids, top_k, True, torch.empty((tokens * top_k, w1.outputs), dtype=x.dtype, device=dev))
+    y = _matvec(hidden, w2, ids, 1, False, torch.empty((tokens * top_k, w2.outputs), dtype=torch.float32, device=dev))
+    out = torch.empty((tokens, w2.outputs), dtype=x.dtype, device=dev)
+    with _lib.on_device(dev):
+        rc = _lib.load().stk_b200_int4_combine(
+            _lib.ptr(y), _lib.ptr(ids), _lib.ptr(weights), _lib.ptr(out), tokens, top_k, w2.num_experts, w2.outputs,
+            _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
+    _lib.check(rc, "stk_b200_int4_combine")
+    return out
