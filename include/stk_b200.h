@@ -410,9 +410,11 @@ int stk_b200_ep_return(const void* result, const int64_t* tags, const uint64_t* 
  * unsort_backward: the gradients of the weighted sum_rows: drows [n_rows, hidden] (zeros in padding) and
  *   dweights [tokens, top_k]; either may be NULL.  Rows are of any length and 16-bit or 32-bit floats.
  * int4_matvec: out[slot] = W_e x[slot / x_div] for e = ids[slot], W = (code - zero) * scale; zeros for slots
- *   without an expert.  words / scales / zeros: as laid out by stk_b200.dmoe.pack_int4 (see
- *   int4_sm100.cuh); zeros NULL: 8 everywhere.  dtype: of x and scales; out: the same type or, with
- *   out_f32, float.  gelu: the exact GeLU of the product.  group 32, 64 or 128.
+ *   without an expert.  records: [experts][outputs / 32][inputs / 128] (rounded up) of
+ *   int4_record_bytes each, as laid out by stk_b200.dmoe.pack_int4 (see int4_sm100.cuh); zeros: whether they
+ *   hold zero points (8 everywhere otherwise).  dtype: of x and the scales; out: the same type or, with
+ *   out_f32, float.  gelu: the GeLU of the product.  group 32, 64 or 128; at most 512 groups
+ *   of inputs and 1024 experts.
  * int4_combine: out[t] = sum_j weights[slot] * y[slot] over the slots of token t that have an expert.
  */
 int stk_b200_top_k_gate(const void* logits, int64_t ld, int64_t tokens, int experts, int top_k, int score,
@@ -433,9 +435,10 @@ int stk_b200_unsort_backward(const void* dout, int64_t ld_dout, const void* rows
                              const float* weights, const int32_t* index, const int32_t* position, void* drows,
                              float* dweights, int64_t tokens, int top_k, int64_t n_rows, int64_t hidden, int dtype,
                              void* stream);
-int stk_b200_int4_matvec(const void* words, const void* scales, const uint8_t* zeros, const void* x,
-                         const int32_t* ids, void* out, int64_t slots, int x_div, int experts, int64_t outputs,
-                         int64_t inputs, int group, int gelu, int out_f32, int dtype, void* stream);
+size_t stk_b200_int4_record_bytes(int group, int zeros);
+int stk_b200_int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots, int x_div,
+                         int experts, int64_t outputs, int64_t inputs, int group, int zeros, int gelu, int out_f32,
+                         int dtype, void* stream);
 int stk_b200_int4_combine(const float* y, const int32_t* ids, const float* weights, void* out, int64_t tokens,
                           int top_k, int experts, int64_t outputs, int dtype, void* stream);
 

@@ -81,8 +81,9 @@ SIGNATURES = {
     "stk_b200_sum_rows": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_i64, _c_int, _c_ptr]),
     "stk_b200_unsort_backward": (_c_int, [_c_ptr, _c_i64, _c_ptr, _c_i64, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                                           _c_i64, _c_int, _c_i64, _c_i64, _c_int, _c_ptr]),
-    "stk_b200_int4_matvec": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64,
-                                      _c_i64, _c_int, _c_int, _c_int, _c_int, _c_ptr]),
+    "stk_b200_int4_record_bytes": (_c_size, [_c_int, _c_int]),
+    "stk_b200_int4_matvec": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_i64, _c_int,
+                                      _c_int, _c_int, _c_int, _c_int, _c_ptr]),
     "stk_b200_int4_combine": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_ptr]),
     "stk_b200_ep_return": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_ptr]),
 }

@@ -2,221 +2,528 @@
 // e, W = (code - zero) * scale with a scale (and a zero point, 8 where there is none) for each output row and group of
 // 32, 64 or 128 inputs.
 //
-// The bytes of the chosen experts' weights bound it: a weight is half a byte, so at 6.5 TB/s an SM has to take in 46
+// The bytes of the chosen experts' weights are the floor: a weight is half a byte, so at 6.5 TB/s an SM has to take in 46
 // weights a clock, more than it could convert and multiply on the CUDA cores in 32 bits (three instructions a weight).
-// So the products run as mma.m16n8k16: 16 output rows x 16 inputs of weights against 8 slots, sums in 32 bits.  Codes
-// become 16-bit floats exactly (an exponent is put above them: 128 + q in bf16, 1024 + q in fp16, and 128 + zero or
-// 1024 + zero is subtracted, exactly); the scale multiplies the 32-bit sum of a group.  Nothing is rounded before the
-// result.
+// So the products run as mma.m16n8k16: 16 output rows x 16 inputs of weights against 8 slots, sums in 32 bits.  The A
+// operand is 16 + code, a 16-bit float made by putting an exponent above the code's four bits (exact, one shift and one
+// logical instruction for two weights).  sum (code - zero) x = sum (16 + code) x - (16 + zero) sum x: the sums of the
+// inputs, a table in shared memory made once for each (expert, tile of slots) by products with ones, are where the sum of
+// a group starts from, and the scale multiplies what comes out.  All of it is in 32 bits; nothing is rounded before the
+// result.  (An infinity among the inputs therefore makes a NaN.)
 //
-// Layout (made once, by the host): a strip of 16 output rows x 64 inputs is 512 bytes in the order in which the lanes
+// Layout (made once, by the host): a record holds 32 output rows (two strips of 16) x 128 inputs, in the order in which
+// the kernel reads them.  First the codes, strip by strip, 64 inputs at a time, 512 bytes in the order in which the lanes
 // of a warp hold the A operand: lane (g, t) = (lane / 4, lane % 4) has 16 bytes, word 2h + s of them the weights of rows
-// g and g + 8 for the inputs 32h + 8t + 4s + {0, 1, 2, 3}; nibble 4b + 2p + r: row g + 8r, input 2p + b of the four.  The
-// order of the inputs inside a product is free, so a lane's share of x is 16 contiguous bytes.  A strip is contiguous
-// along the inputs, and every load of a warp is 512 contiguous bytes.
+// g and g + 8 for the inputs 32h + 8t + 4s + {0, 1, 2, 3}; nibble 4b + 2p + r: row g + 8r, input 2p + b of the four.  (The
+// order of the inputs inside a product is free, so a lane's share of x is 16 contiguous bytes.)  A word is turned left by
+// 3 bits (bf16) or 6 (fp16), so that its first two codes lie where a 16-bit float has its last exact bits.  Then the
+// scales [group of the record][strip][g][r], then the zero points in the same order, a byte each.  What is beyond the
+// last row or input is code 0, scale 0, zero point 0: nothing.
+//
+// One CTA of 16 warps per SM takes an equal share of the records' rows (of every expert and tile of up to 16 of its
+// slots), several of them at a time: an item is 1, 2, 4, 8 or 16 of them, as many as are left, so that shares stay equal
+// to a record's rows; 16 / that many warps cut each row along the inputs, and their sums are joined in shared memory, in
+// order.  Each warp streams its records through a ring of its own, by bulk copies that one lane starts; the copies run
+// ahead across the items.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #include "../../include/stk_b200.h"
+#include "bsmm_sm100.cuh"
 #include "gate_sm100.cuh"
+#include "sm100_ptx.cuh"
 #include "status.cuh"
 
 namespace stk {
 
-constexpr int kInt4Threads = 256;
-constexpr int kInt4Warps = kInt4Threads / 32;
+constexpr int kInt4Warps = 16;
+constexpr int kInt4Threads = 32 * kInt4Warps;
+constexpr int kInt4Strips = 2;                      // strips of a record
+constexpr int kInt4Rows = 16 * kInt4Strips;
+constexpr int kInt4Inputs = 128;
+constexpr int kInt4Stages = 2;                      // records of a warp's ring
+constexpr int kInt4MaxExperts = 1024;
+constexpr int kInt4MaxSlots = 256;                  // of one launch
+constexpr int kInt4MaxGroups = 512;                 // of the inputs
+constexpr int kInt4MaxTiles = 2;                    // products of 8 slots per item
+constexpr int kInt4MaxEntries = kInt4MaxSlots;      // (expert, tile) pairs: each holds a slot at least
+
+template <int kGroup>
+struct Int4RecordBase {
+  static constexpr int kGroups = kInt4Inputs / kGroup;
+  uint4 words[kInt4Strips][2][32];
+  uint32_t scales[kGroups][kInt4Strips][8];         // rows g and g + 8
+};
+template <int kGroup, bool kZeros>
+struct Int4Record : Int4RecordBase<kGroup> {};
+template <int kGroup>
+struct Int4Record<kGroup, true> : Int4RecordBase<kGroup> {
+  uint16_t zeros[Int4RecordBase<kGroup>::kGroups][kInt4Strips][8];
+};
+struct Int4Args {
+  const unsigned char* records;  // [experts][outputs / 32][inputs / 128], rounded up
+  const void* x;          // [.., inputs], contiguous
+  const int32_t* ids;     // [slots]
+  void* out;              // [slots][outputs]: T, or float
+  int slots, first_slot;  // slots of this launch; the first one's number
+  int x_div, experts, outputs, inputs;
+  int min_log;            // log2 of the fewest row groups of an item
+  int gelu, out_f32;
+};
+
+constexpr int kInt4MaxLog = 4;                      // log2 of the most rows of records of an item: a warp each
+
+// The items of a CTA, one after the other: rows of records [block, block + n) of an entry, n <= 2^log, 16 >> log warps each.
+struct Int4Item {
+  int left;                // rows of records of the CTA's share from this item on
+  int entry, block, n, log;
+  int c0, c1, row;         // the warp's part: these records of this row (from `block` on)
+  __device__ __forceinline__ void settle(const Int4Args& a, int blocks, int units, int warp) {
+    n = min(left, blocks - block);
+    log = kInt4MaxLog;
+    static_assert(kInt4Warps == 1 << kInt4MaxLog, "");
+    while (log > a.min_log && (1 << log) > n) --log;
+    n = min(n, 1 << log);
+    const int split_log = kInt4MaxLog - log, share = warp & ((1 << split_log) - 1);
+    row = warp >> split_log;
+    c0 = units * share >> split_log;
+    c1 = row < n ? units * (share + 1) >> split_log : c0;
+  }
+  __device__ __forceinline__ bool next(const Int4Args& a, int blocks, int units, int warp) {
+    left -= n;
+    block += n;
+    if (block == blocks) {
+      block = 0;
+      ++entry;
+    }
+    if (left <= 0) return false;
+    settle(a, blocks, units, warp);
+    return true;
+  }
+};
+
+// Where a warp's copies have got to.
+struct Int4Cursor {
+  const unsigned char* record;  // the next one
+  int more;                     // of the item still to be copied
+  uint32_t head;                // copied so far; the next one goes to stage head % kInt4Stages
+  int left, entry, block;       // the items after it
+};
+
+template <int kGroup, bool kZeros>
+struct Int4Smem {
+  Int4Record<kGroup, kZeros> ring[kInt4Warps][kInt4Stages];
+  float joined[kInt4Warps][kInt4Strips * kInt4MaxTiles * 4][32];
+  uint64_t full[kInt4Warps][kInt4Stages];
+  int32_t list[kInt4MaxSlots];                      // slots, expert by expert
+  int32_t row[kInt4MaxSlots];                       // their rows of x
+  uint16_t entry_expert[kInt4MaxEntries];
+  uint16_t entry_first[kInt4MaxEntries];            // in the list
+  uint16_t entry_slots[kInt4MaxEntries];
+  int32_t counter[kInt4MaxExperts];
+  int32_t entries;
+  int32_t dropped;
+  int32_t stuck;
+  alignas(16) float sums[1];                        // [groups][8 * kInt4MaxTiles]: of the entry's slots' inputs
+};
 
 template <typename T> struct Int4Type;
 template <> struct Int4Type<__nv_bfloat16> {
-  using Pair = __nv_bfloat162;
-  static constexpr uint32_t kMagic = 0x43004300u;  // 128: one step is 1
-  static constexpr float kBase = 128.0f;
-  __device__ static Pair pair(float v) { return __float2bfloat162_rn(v); }
+  static constexpr uint32_t kMagic = 0x41804180u;  // 16, with steps of 1 from bit 3 on
+  static constexpr int kBit = 3;
+  static constexpr uint32_t kOnes = 0x3f803f80u;
+  __device__ static float2 pair(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
   __device__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  __device__ static void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+  }
 };
 template <> struct Int4Type<__half> {
-  using Pair = __half2;
-  static constexpr uint32_t kMagic = 0x64006400u;  // 1024: one step is 1
-  static constexpr float kBase = 1024.0f;
-  __device__ static Pair pair(float v) { return __float2half2_rn(v); }
+  static constexpr uint32_t kMagic = 0x4c004c00u;  // 16, with steps of 1 from bit 6 on
+  static constexpr int kBit = 6;
+  static constexpr uint32_t kOnes = 0x3c003c00u;
+  __device__ static float2 pair(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   __device__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
+  __device__ static void mma_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, const float (&c)[4]) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+  }
 };
 
-// The 8 weights of one word, as the A operand of one product; zero_lo / zero_hi: base + zero point of rows g, g + 8.
+// 16 + code for the 8 codes of a word, as the A operand of one product.  mask and magic are registers (int4_constant):
+// one logical instruction takes one immediate, and with two constants known to it the compiler makes two of it (14
+// instead of 7 integer instructions a word).
 template <typename T>
-__device__ __forceinline__ void int4_decode(uint32_t w, typename Int4Type<T>::Pair zero_lo,
-                                            typename Int4Type<T>::Pair zero_hi, uint32_t (&a)[4]) {
-  using Pair = typename Int4Type<T>::Pair;
+__device__ __forceinline__ void int4_decode(uint32_t w, uint32_t mask, uint32_t magic, uint32_t (&a)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t bits = ((w >> (4 * i)) & 0x000f000fu) | Int4Type<T>::kMagic;
-    const Pair v = __hsub2(*reinterpret_cast<const Pair*>(&bits), i & 1 ? zero_hi : zero_lo);
-    a[i] = *reinterpret_cast<const uint32_t*>(&v);
+  for (int i = 0; i < 4; ++i)
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(a[i]) : "r"(__funnelshift_r(w, w, 4 * i)), "r"(mask), "r"(magic));
+}
+__device__ __forceinline__ uint32_t int4_constant(uint32_t v) {
+  uint32_t r;
+  asm volatile("mov.b32 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+// The products' epilogue's GeLU; a NaN stays one.
+__device__ __forceinline__ float int4_gelu(float x) { return x == x ? gelu_erf(x) : x; }
+
+__device__ __forceinline__ void int4_copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(to), "l"(from), "r"(bytes), "r"(bar) : "memory");
+}
+
+// To the first record of the next item in which the warp has a part.
+template <int kGroup, bool kZeros>
+__device__ __forceinline__ void int4_point(const Int4Args& a, const Int4Smem<kGroup, kZeros>& sm, int blocks, int units,
+                                           int warp, Int4Cursor& c) {
+  Int4Item item;
+  while (c.left > 0) {
+    item.left = c.left;
+    item.block = c.block;
+    item.settle(a, blocks, units, warp);
+    const int64_t row = static_cast<int64_t>(sm.entry_expert[c.entry]) * blocks + c.block + item.row;
+    c.left -= item.n;
+    c.block += item.n;
+    if (c.block == blocks) {
+      c.block = 0;
+      ++c.entry;
+    }
+    if (item.c0 >= item.c1) continue;
+    c.record = a.records + (row * units + item.c0) * static_cast<int64_t>(sizeof(Int4Record<kGroup, kZeros>));
+    c.more = item.c1 - item.c0;
+    return;
   }
 }
 
-// x Phi(x), Phi from the complementary error function: no difference of nearly equal numbers on the negative side, and a
-// NaN stays one.  (A few thousand values a product: its cost does not show.)
-__device__ __forceinline__ float int4_gelu(float x) { return 0.5f * x * erfcf(-0.70710678118654752f * x); }
+// Starts the next copy; every lane has read the stage that it goes to.
+template <int kGroup, bool kZeros>
+__device__ __forceinline__ void int4_fetch(const Int4Args& a, Int4Smem<kGroup, kZeros>& sm, int blocks, int units, int warp,
+                                           int lane, Int4Cursor& c) {
+  constexpr uint32_t kBytes = sizeof(Int4Record<kGroup, kZeros>);
+  static_assert(kBytes % 16 == 0 && kBytes == 2048 + kInt4Inputs / kGroup * kInt4Rows * (kZeros ? 3 : 2), "bulk copies");
+  if (c.more == 0) return;
+  if (lane == 0) {
+    const uint32_t bar = smem_u32(&sm.full[warp][c.head % kInt4Stages]);
+    mbar_arrive_expect_tx(bar, kBytes);
+    int4_copy(smem_u32(&sm.ring[warp][c.head % kInt4Stages]), c.record, kBytes, bar);
+  }
+  ++c.head;
+  c.record += kBytes;
+  if (--c.more == 0) int4_point<kGroup, kZeros>(a, sm, blocks, units, warp, c);
+}
 
-struct Int4Args {
-  const uint4* words;     // [experts][strips][chunks][32]
-  const void* scales;     // [experts][strips][groups][16]
-  const uint8_t* zeros;   // the same, or NULL
-  const void* x;          // [.., inputs], contiguous
-  const int32_t* ids;     // [slots]
-  void* out;              // [slots][outputs]: T, or float
-  int64_t slots;
-  int x_div, experts, outputs, inputs, group;
-  int split;              // warps that share a strip
-  int by_slot;            // grid.y goes by slots (first use of an expert) instead of experts
-  int gelu, out_f32;
+// x of the entry's slots as the lanes hold the B operand: 8 inputs of slot 8 n + g.
+template <typename T, int NT, int kGroup, bool kZeros>
+struct Int4Inputs {
+  const T* x[NT];
+  __device__ __forceinline__ Int4Inputs(const Int4Args& a, const Int4Smem<kGroup, kZeros>& sm, int first, int slots, int c,
+                                        int lane) {
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+      // (columns beyond the slots repeat the last one: a column of a product does not reach the others)
+      x[n] = static_cast<const T*>(a.x) + static_cast<int64_t>(sm.row[first + min(8 * n + lane / 4, slots - 1)]) * a.inputs +
+             c * kInt4Inputs + 8 * (lane % 4);
+  }
+  __device__ __forceinline__ void next() {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x[n] += kInt4Inputs;
+  }
+  // A quarter, of 32 inputs, of record c, which x is at.  (One beyond the inputs has codes, scales and zero points of 0:
+  // any of the row's values will do.  A choice between loaded values and zeros would wait for the load where it stands.)
+  __device__ __forceinline__ void load(const Int4Args& a, int c, int quarter, uint4 (&to)[NT]) const {
+    const int at = kGroup == 128 || c * kInt4Inputs + quarter * 32 < a.inputs ? 4 * quarter : 0;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) to[n] = __ldg(reinterpret_cast<const uint4*>(x[n]) + at);
+  }
 };
 
-// A CTA: kInt4Warps / split strips of one expert, against the slots that chose it, 8 * NT at a time.
-template <typename T, int NT>
-__global__ void __launch_bounds__(kInt4Threads, 2)
-int4_matvec_kernel(const Int4Args a) {
-  constexpr int kTile = 8 * NT;
-  __shared__ int32_t list[kInt4Threads];
-  __shared__ int found[kInt4Warps + 1];
-  __shared__ float joined[kInt4Warps][NT * 4][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  const int strips = (a.outputs + 15) / 16, chunks = (a.inputs + 63) / 64, groups = a.inputs / a.group;
-  const int per_cta = kInt4Warps / a.split;
-  const int strip = blockIdx.x * per_cta + warp / a.split, part = warp % a.split;
-  int expert = blockIdx.y;
-  if (a.by_slot) {
-    expert = a.ids[blockIdx.y];
-    for (int64_t s = 0; s < blockIdx.y; ++s)
-      if (a.ids[s] == expert) return;              // an earlier slot's CTA has this expert
-  }
-  if (expert < 0 || expert >= a.experts) {         // the slots without an expert: zeros
-    const int n0 = blockIdx.x * per_cta * 16, n1 = min(a.outputs, n0 + per_cta * 16);
-    for (int64_t s = 0; s < a.slots; ++s) {
-      const int e = a.ids[s];
-      if (e >= 0 && e < a.experts) continue;
-      if (e >= a.experts && blockIdx.x == 0 && threadIdx.x == 0) report_status(STK_ERR_BAD_DIMS);
-      for (int n = n0 + threadIdx.x; n < n1; n += kInt4Threads) {
-        if (a.out_f32) static_cast<float*>(a.out)[s * a.outputs + n] = 0.0f;
-        else static_cast<T*>(a.out)[s * a.outputs + n] = from_f32<T>(0.0f);
-      }
-    }
-    return;
-  }
-  const int per = (chunks + a.split - 1) / a.split;
-  const int c0 = part * per, c1 = min(chunks, c0 + per);
-  const bool busy = strip < strips;
-  const int64_t at_strip = static_cast<int64_t>(expert) * strips + (busy ? strip : 0);
-  const uint4* words = a.words + at_strip * chunks * 32 + lane;
-  const T* scales = static_cast<const T*>(a.scales) + at_strip * groups * 16 + g;
-  const uint8_t* zeros = a.zeros == nullptr ? nullptr : a.zeros + at_strip * groups * 16 + g;
-
-  for (int64_t window = 0; window < a.slots; window += kInt4Threads) {
-    // the window's slots of this expert, in order
-    const int64_t s = window + threadIdx.x;
-    const bool mine = s < a.slots && a.ids[s] == expert;
-    const unsigned votes = __ballot_sync(0xffffffffu, mine);
-    __syncthreads();
-    if (lane == 0) found[warp] = __popc(votes);
-    __syncthreads();
-    int before = 0, n_slots = 0;
-    for (int w = 0; w < kInt4Warps; ++w) {
-      before += w < warp ? found[w] : 0;
-      n_slots += found[w];
-    }
-    if (mine) list[before + __popc(votes & ((1u << lane) - 1))] = static_cast<int32_t>(s);
-    __syncthreads();
-    for (int tile = 0; tile < n_slots; tile += kTile) {
-      float acc[NT][4];
-      const T* x[NT];
+// The table of an entry's sums of inputs, a group each; without zero points, -(16 + 8) times them.
+template <typename T, int NT, int kGroup, bool kZeros>
+__device__ __forceinline__ void int4_sums(const Int4Args& a, Int4Smem<kGroup, kZeros>& sm, int entry, int units, int warp,
+                                          int lane) {
+  const uint32_t ones[4] = {Int4Type<T>::kOnes, Int4Type<T>::kOnes, Int4Type<T>::kOnes, Int4Type<T>::kOnes};
+  constexpr int kPer = kGroup / 32;
+  for (int c = warp; c < units; c += kInt4Warps) {
+    const Int4Inputs<T, NT, kGroup, kZeros> in(a, sm, sm.entry_first[entry], sm.entry_slots[entry], c, lane);
+    uint4 v[4][NT];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) in.load(a, c, h, v[h]);
+    float sum[NT][4];
+#pragma unroll
+    for (int h = 0; h < 4; ++h) {
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
-        const int which = tile + 8 * n + g;
-        x[n] = which < n_slots ? static_cast<const T*>(a.x) + static_cast<int64_t>(list[which] / a.x_div) * a.inputs + 8 * t : nullptr;
+        if (h % kPer == 0) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.0f;
+        Int4Type<T>::mma(sum[n], ones, v[h][n].x, v[h][n].y);
+        Int4Type<T>::mma(sum[n], ones, v[h][n].z, v[h][n].w);
+        const int group = c * (kInt4Inputs / kGroup) + h / kPer;
+        if (h % kPer == kPer - 1 && lane < 4) {       // (every row of the product is the sum)
+          float* to = &sm.sums[(group * kInt4MaxTiles + n) * 8 + 2 * lane];
+          to[0] = kZeros ? sum[n][0] : -24.0f * sum[n][0];
+          to[1] = kZeros ? sum[n][1] : -24.0f * sum[n][1];
+        }
       }
-      if (busy) {
-#pragma unroll 4
-        for (int c = c0; c < c1; ++c) {
-          const uint4 q = __ldcs(words + static_cast<int64_t>(c) * 32);
-          const uint32_t word[4] = {q.x, q.y, q.z, q.w};
+    }
+  }
+}
+
+// The warp's part of an item: records [c0, c1), from the ring's stage tail % kInt4Stages on; NT tiles of 8 slots.
+// before: the last item's log.
+template <typename T, int NT, int kGroup, bool kZeros>
+__device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZeros>& sm, const Int4Item& item, int blocks,
+                                          int units, int warp, int lane, uint32_t& tail, int& before, Int4Cursor& cursor) {
+  const int g = lane >> 2, t = lane & 3, c0 = item.c0, c1 = item.c1;
+  const int first = sm.entry_first[item.entry], slots = sm.entry_slots[item.entry];
+  Int4Inputs<T, NT, kGroup, kZeros> in(a, sm, first, slots, c0, lane);
+  float acc[kInt4Strips][NT][4], part[kInt4Strips][NT][4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k0 = c * 64 + h * 32;
-            if (k0 >= a.inputs) break;
-            uint4 xb[NT];
+  for (int r = 0; r < kInt4Strips; ++r)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-              xb[n] = x[n] != nullptr ? __ldg(reinterpret_cast<const uint4*>(x[n] + k0)) : make_uint4(0, 0, 0, 0);
-            const int at = k0 / a.group * 16;
-            const float scale_lo = to_f32(scales[at]), scale_hi = to_f32(scales[at + 8]);
-            const auto zero_lo = Int4Type<T>::pair(Int4Type<T>::kBase + (zeros != nullptr ? zeros[at] : 8));
-            const auto zero_hi = Int4Type<T>::pair(Int4Type<T>::kBase + (zeros != nullptr ? zeros[at + 8] : 8));
-            float part_sum[NT][4];
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+      for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
+  const uint32_t mask = int4_constant(0x000f000fu << Int4Type<T>::kBit), magic = int4_constant(Int4Type<T>::kMagic);
+  // x runs kAhead quarters (of 32 inputs) ahead, across the records
+  constexpr int kAhead = NT == 1 ? 4 : 2;
+  uint4 xq[kAhead][NT];
+  if (c0 < c1) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) part_sum[n][i] = 0.0f;
+    for (int h = 0; h < kAhead; ++h) in.load(a, c0, h, xq[h]);
+  }
+  const float* sums = sm.sums + c0 * (kInt4Inputs / kGroup) * kInt4MaxTiles * 8 + 2 * t;
+  for (int c = c0; c < c1; ++c) {
+    const uint32_t from = tail % kInt4Stages;
+    const Int4Record<kGroup, kZeros>& st = sm.ring[warp][from];
+    if (!mbar_wait(smem_u32(&sm.full[warp][from]), tail / kInt4Stages & 1u, &sm.stuck)) {
+      report_status(STK_ERR_DEVICE_TIMEOUT);
+      cursor.more = cursor.left = 0;                 // no further copies
+    }
+    uint4 q[kInt4Strips];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              uint32_t w[4];
-              int4_decode<T>(word[2 * h + u], zero_lo, zero_hi, w);
+    for (int h = 0; h < 4; ++h) {                    // quarters
+      constexpr int kPer = kGroup / 32;
+      if (h % 2 == 0) {
 #pragma unroll
-              for (int n = 0; n < NT; ++n)
-                Int4Type<T>::mma(part_sum[n], w, u ? xb[n].z : xb[n].x, u ? xb[n].w : xb[n].y);
+        for (int r = 0; r < kInt4Strips; ++r) q[r] = st.words[r][h / 2][lane];
+      }
+      float2 sum[NT];
+      if (h % kPer == 0) {                           // a new group
+#pragma unroll
+        for (int n = 0; n < NT; ++n) sum[n] = *reinterpret_cast<const float2*>(sums + (h / kPer * kInt4MaxTiles + n) * 8);
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int r = 0; r < kInt4Strips; ++r) {
+          uint32_t w[4];
+          int4_decode<T>(h % 2 ? (u ? q[r].w : q[r].z) : (u ? q[r].y : q[r].x), mask, magic, w);
+          float zero_lo = 1.0f, zero_hi = 1.0f;
+          if constexpr (kZeros) {
+            if (h % kPer == 0 && u == 0) {
+              const uint32_t z = st.zeros[h / kPer][r][g];
+              zero_lo = -16.0f - static_cast<float>(z & 0xffu);
+              zero_hi = -16.0f - static_cast<float>(z >> 8);
             }
+          }
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            const uint4& v = xq[h % kAhead][n];
+            if (h % kPer == 0 && u == 0) {
+              float start[4] = {sum[n].x, sum[n].y, sum[n].x, sum[n].y};
+              if (kZeros) {
 #pragma unroll
-              for (int i = 0; i < 4; ++i) acc[n][i] = fmaf(i < 2 ? scale_lo : scale_hi, part_sum[n][i], acc[n][i]);
+                for (int i = 0; i < 4; ++i) start[i] *= i < 2 ? zero_lo : zero_hi;
+              }
+              Int4Type<T>::mma_from(part[r][n], w, v.x, v.y, start);
+            } else {
+              Int4Type<T>::mma(part[r][n], w, u ? v.z : v.x, u ? v.w : v.y);
+            }
           }
         }
       }
-      if (a.split > 1) {                             // the parts of a strip, joined in order
-        __syncthreads();
-        if (part != 0) {
+      if (h == 4 - kAhead) in.next();
+      if (h + kAhead < 4) in.load(a, c, h + kAhead, xq[h % kAhead]);
+      else if (c + 1 < c1) in.load(a, c + 1, h + kAhead - 4, xq[h % kAhead]);
+      if (h % kPer == kPer - 1) {                    // the end of a group
+#pragma unroll
+        for (int r = 0; r < kInt4Strips; ++r) {
+          const float2 scale = Int4Type<T>::pair(st.scales[h / kPer][r][g]);
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) joined[warp][n * 4 + i][lane] = acc[n][i];
-        }
-        __syncthreads();
-        if (part == 0) {
-          for (int p = 1; p < a.split; ++p)
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) acc[n][i] += joined[warp + p][n * 4 + i][lane];
+            for (int i = 0; i < 4; ++i) acc[r][n][i] = fmaf(i < 2 ? scale.x : scale.y, part[r][n][i], acc[r][n][i]);
         }
       }
-      if (part == 0 && busy) {
+    }
+    sums += kInt4Inputs / kGroup * kInt4MaxTiles * 8;
+    ++tail;
+    __syncwarp();                                    // the record is read: the copies run on into its stage
+    int4_fetch<kGroup, kZeros>(a, sm, blocks, units, warp, lane, cursor);
+  }
+  // The sums of a row's warps are added up, in order, each warp taking its share of the values, between barriers of the
+  // row's warps (before the first of them they read the last item's sums; where rows get fewer warps, those were a larger
+  // group's, and the barrier is the whole CTA's).  Groups of each size have barriers of their own (0 for one group, 1 - 2,
+  // 3 - 6, 7 - 14): some warps may be an item ahead, in groups of another size.
+  constexpr int kValues = kInt4Strips * NT * 4;
+  const int split_log = kInt4MaxLog - item.log, split = 1 << split_log;
+  const auto meet = [&] {
+    if (split_log == 0) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"((1 << item.log) - 1 + item.row), "r"(32 * split) : "memory");
+  };
+  if (item.log > before) __syncthreads();
+  else meet();
+  before = item.log;
+  float (*mine)[32] = sm.joined[warp];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+  for (int r = 0; r < kInt4Strips; ++r)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int which = tile + 8 * n + 2 * t + (i & 1), row = strip * 16 + g + (i >= 2 ? 8 : 0);
-            if (which >= n_slots || row >= a.outputs) continue;
-            const int64_t at = static_cast<int64_t>(list[which]) * a.outputs + row;
-            const float v = a.gelu ? int4_gelu(acc[n][i]) : acc[n][i];
-            if (a.out_f32) static_cast<float*>(a.out)[at] = v;
-            else static_cast<T*>(a.out)[at] = from_f32<T>(v);
-          }
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mine[(r * NT + n) * 4 + i][lane] = acc[r][n][i];
+  meet();
+  if (item.row < item.n) {
+    const int row0 = (item.block + item.row) * kInt4Rows + g;
+    const float (*group)[kInt4Strips * kInt4MaxTiles * 4][32] = &sm.joined[item.row << split_log];
+    for (int v = warp & (split - 1); v < kValues; v += split) {
+      const int i = v % 4, n = v / 4 % NT, r = v / 4 / NT;
+      const int which = 8 * n + 2 * t + i % 2, row = row0 + r * 16 + i / 2 * 8;
+      if (which >= slots || row >= a.outputs) continue;
+      float s = 0.0f;
+      for (int p = 0; p < split; ++p) s += group[p][v][lane];
+      const int64_t at = static_cast<int64_t>(sm.list[first + which] + a.first_slot) * a.outputs + row;
+      s = a.gelu ? int4_gelu(s) : s;
+      if (a.out_f32) static_cast<float*>(a.out)[at] = s;
+      else static_cast<T*>(a.out)[at] = from_f32<T>(s);
+    }
+  }
+}
+
+template <typename T, int kGroup, bool kZeros>
+__global__ void __launch_bounds__(kInt4Threads, 1)
+int4_matvec_kernel(const Int4Args a) {
+  extern __shared__ __align__(16) unsigned char int4_smem[];
+  using Smem = Int4Smem<kGroup, kZeros>;
+  Smem& sm = *reinterpret_cast<Smem*>(int4_smem);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int32_t* ids = a.ids + a.first_slot;
+
+  // the slots, expert by expert, and the (expert, tile) entries of up to 8 * kInt4MaxTiles of them
+  for (int e = threadIdx.x; e < a.experts; e += kInt4Threads) sm.counter[e] = 0;
+  if (threadIdx.x == 0) sm.dropped = sm.stuck = 0;
+  if (threadIdx.x < kInt4Warps * kInt4Stages) mbar_init(smem_u32(&sm.full[0][0] + threadIdx.x), 1);
+  fence_barrier_init();
+  __syncthreads();
+  for (int s = threadIdx.x; s < a.slots; s += kInt4Threads) {
+    const int e = ids[s];
+    if (e >= 0 && e < a.experts) atomicAdd(&sm.counter[e], 1);
+    else sm.dropped = 1;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    constexpr int kTile = 8 * kInt4MaxTiles;
+    int slots_before = 0, entries_before = 0;
+    for (int e0 = 0; e0 < a.experts; e0 += 32) {
+      const int e = e0 + lane;
+      const int n = e < a.experts ? sm.counter[e] : 0, tiles = (n + kTile - 1) / kTile;
+      int slots_up = n, tiles_up = tiles;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, slots_up, off), v = __shfl_up_sync(0xffffffffu, tiles_up, off);
+        if (lane >= off) {
+          slots_up += u;
+          tiles_up += v;
+        }
+      }
+      int first = slots_before + slots_up - n, entry = entries_before + tiles_up - tiles;
+      if (e < a.experts) sm.counter[e] = first;
+      for (int left = n; left > 0; left -= kTile, first += kTile, ++entry) {
+        sm.entry_expert[entry] = static_cast<uint16_t>(e);
+        sm.entry_first[entry] = static_cast<uint16_t>(first);
+        sm.entry_slots[entry] = static_cast<uint16_t>(min(left, kTile));
+      }
+      slots_before += __shfl_sync(0xffffffffu, slots_up, 31);
+      entries_before += __shfl_sync(0xffffffffu, tiles_up, 31);
+    }
+    if (lane == 0) sm.entries = entries_before;
+  }
+  __syncthreads();
+  if (warp == 0) {                                   // in order: every CTA has to cut the same tiles
+    for (int s0 = 0; s0 < a.slots; s0 += 32) {
+      const int s = s0 + lane, id = s < a.slots ? ids[s] : -1, e = id < a.experts ? id : -1;
+      const unsigned same = __match_any_sync(0xffffffffu, e), before = same & ((1u << lane) - 1);
+      const int at = e >= 0 ? sm.counter[e] + __popc(before) : 0;
+      __syncwarp();
+      if (e >= 0) {
+        sm.list[at] = s;
+        sm.row[at] = (s + a.first_slot) / a.x_div;
+        if (before == 0) sm.counter[e] = at + __popc(same);
+      }
+      __syncwarp();
+    }
+  }
+  __syncthreads();
+  if (sm.dropped) {                                  // zeros for the slots without an expert, dealt out to the CTAs
+    for (int s = blockIdx.x; s < a.slots; s += gridDim.x) {
+      const int e = ids[s];
+      if (e >= 0 && e < a.experts) continue;
+      if (e >= a.experts && threadIdx.x == 0) report_status(STK_ERR_BAD_DIMS);
+      const int64_t at = static_cast<int64_t>(s + a.first_slot) * a.outputs;
+      for (int n = threadIdx.x; n < a.outputs; n += kInt4Threads) {
+        if (a.out_f32) static_cast<float*>(a.out)[at + n] = 0.0f;
+        else static_cast<T*>(a.out)[at + n] = from_f32<T>(0.0f);
       }
     }
   }
+
+  const int blocks = (a.outputs + kInt4Rows - 1) / kInt4Rows, units = (a.inputs + kInt4Inputs - 1) / kInt4Inputs;
+  const int64_t rows = static_cast<int64_t>(sm.entries) * blocks;
+  const int64_t row0 = rows * blockIdx.x / gridDim.x, row1 = rows * (blockIdx.x + 1) / gridDim.x;
+  if (row0 >= row1) return;
+  Int4Item item;
+  item.left = static_cast<int>(row1 - row0);
+  item.entry = static_cast<int>(row0 / blocks);
+  item.block = static_cast<int>(row0 - static_cast<int64_t>(item.entry) * blocks);
+  item.settle(a, blocks, units, warp);
+
+  Int4Cursor cursor;
+  cursor.left = item.left;
+  cursor.entry = item.entry;
+  cursor.block = item.block;
+  cursor.more = 0;
+  cursor.head = 0;
+  int4_point<kGroup, kZeros>(a, sm, blocks, units, warp, cursor);
+#pragma unroll 1
+  for (int i = 0; i < kInt4Stages; ++i) int4_fetch<kGroup, kZeros>(a, sm, blocks, units, warp, lane, cursor);
+  int before = kInt4MaxLog, entry = -1;
+  uint32_t tail = 0;
+  do {
+    const bool wide = sm.entry_slots[item.entry] > 8;
+    if (item.entry != entry) {
+      entry = item.entry;
+      __syncthreads();                               // nobody reads the last entry's table any more
+      if (wide) int4_sums<T, 2, kGroup, kZeros>(a, sm, entry, units, warp, lane);
+      else int4_sums<T, 1, kGroup, kZeros>(a, sm, entry, units, warp, lane);
+      __syncthreads();
+    }
+    if (wide) int4_item<T, 2, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
+    else int4_item<T, 1, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
+  } while (item.next(a, blocks, units, warp));
 }
 
 // out[t] = sum_j weights[t, j] * y[t * k + j] over the choices that have an expert; y in 32 bits.
@@ -237,51 +544,71 @@ int4_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids
   out[i] = from_f32<T>(acc);
 }
 
-static int int4_sms() {
+template <typename T, int kGroup, bool kZeros>
+static int int4_launch(Int4Args a, int64_t slots, cudaStream_t stream) {
   static int sms[64] = {};
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return STK_ERR_LAUNCH;
+  const auto kernel = int4_matvec_kernel<T, kGroup, kZeros>;
+  const auto bytes = [](int units) {
+    return sizeof(Int4Smem<kGroup, kZeros>) + static_cast<size_t>(units) * (kInt4Inputs / kGroup) * kInt4MaxTiles * 8 * sizeof(float);
+  };
+  constexpr int kMaxUnits = kInt4MaxGroups * kGroup / kInt4Inputs;
   if (sms[dev] == 0) {
     int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return -1;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0 ||
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes(kMaxUnits))) != cudaSuccess) {
+      cudaGetLastError();
+      return STK_ERR_LAUNCH;
+    }
     sms[dev] = n;
   }
-  return sms[dev];
+  const int units = (a.inputs + kInt4Inputs - 1) / kInt4Inputs;
+  a.min_log = 0;                                      // no more warps along the inputs than there are records
+  while ((kInt4Warps >> a.min_log) > units) ++a.min_log;
+  for (int64_t first = 0; first < slots; first += kInt4MaxSlots) {
+    a.first_slot = static_cast<int>(first);
+    a.slots = static_cast<int>(slots - first < kInt4MaxSlots ? slots - first : kInt4MaxSlots);
+    kernel<<<static_cast<unsigned>(sms[dev]), kInt4Threads, bytes(units), stream>>>(a);
+    if (cudaGetLastError() != cudaSuccess) return STK_ERR_LAUNCH;
+  }
+  return STK_OK;
 }
-
 template <typename T>
-static int int4_launch(Int4Args a, cudaStream_t stream) {
-  const int sms = int4_sms();
-  if (sms <= 0) return STK_ERR_LAUNCH;
-  const int64_t strips = (a.outputs + 15) / 16, chunks = (a.inputs + 63) / 64;
-  a.by_slot = a.slots < a.experts;
-  const int64_t y = a.by_slot ? a.slots : a.experts + 1;
-  a.split = 1;
-  while (a.split < kInt4Warps && a.split * 2 <= chunks && strips * (a.by_slot ? a.slots : a.experts) * a.split < sms * 16) a.split *= 2;
-  const int64_t per_cta = kInt4Warps / a.split;
-  const dim3 grid(static_cast<unsigned>((strips + per_cta - 1) / per_cta), static_cast<unsigned>(y));
-  if (a.slots <= 4 * static_cast<int64_t>(a.experts)) int4_matvec_kernel<T, 1><<<grid, kInt4Threads, 0, stream>>>(a);
-  else int4_matvec_kernel<T, 2><<<grid, kInt4Threads, 0, stream>>>(a);
-  return cudaGetLastError() == cudaSuccess ? STK_OK : STK_ERR_LAUNCH;
+static int int4_by_group(const Int4Args& a, int group, int zeros, int64_t slots, cudaStream_t stream) {
+  if (!zeros) {
+    if (group == 32) return int4_launch<T, 32, false>(a, slots, stream);
+    if (group == 64) return int4_launch<T, 64, false>(a, slots, stream);
+    return int4_launch<T, 128, false>(a, slots, stream);
+  }
+  if (group == 32) return int4_launch<T, 32, true>(a, slots, stream);
+  if (group == 64) return int4_launch<T, 64, true>(a, slots, stream);
+  return int4_launch<T, 128, true>(a, slots, stream);
 }
 
 }  // namespace stk
 
-extern "C" int stk_b200_int4_matvec(const void* words, const void* scales, const uint8_t* zeros, const void* x,
-                                    const int32_t* ids, void* out, int64_t slots, int x_div, int experts,
-                                    int64_t outputs, int64_t inputs, int group, int gelu, int out_f32, int dtype,
-                                    void* stream) {
+extern "C" size_t stk_b200_int4_record_bytes(int group, int zeros) {
+  if (group != 32 && group != 64 && group != 128) return 0;
+  return 2048 + static_cast<size_t>(stk::kInt4Inputs / group) * stk::kInt4Rows * (zeros ? 3 : 2);
+}
+
+extern "C" int stk_b200_int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots,
+                                    int x_div, int experts, int64_t outputs, int64_t inputs, int group, int zeros,
+                                    int gelu, int out_f32, int dtype, void* stream) {
   if (slots < 0 || x_div < 1 || experts < 1 || outputs < 1 || inputs < 1) return STK_ERR_BAD_DIMS;
   if ((group != 32 && group != 64 && group != 128) || inputs % group) return STK_ERR_BAD_DIMS;
   if (dtype != STK_F16 && dtype != STK_BF16) return STK_ERR_BAD_DTYPE;
-  if (slots > INT32_MAX || outputs > (1 << 24) || inputs > (1 << 24) || experts > 65534) return STK_ERR_TOO_LARGE;
+  if (slots > INT32_MAX || outputs > (1 << 20) || inputs / group > stk::kInt4MaxGroups || experts > stk::kInt4MaxExperts)
+    return STK_ERR_TOO_LARGE;
   if (slots == 0) return STK_OK;
-  if (!words || !scales || !x || !ids || !out) return STK_ERR_NULL_POINTER;
-  if ((reinterpret_cast<uintptr_t>(words) | reinterpret_cast<uintptr_t>(x)) % 16) return STK_ERR_BAD_LAYOUT;
-  stk::Int4Args a{static_cast<const uint4*>(words), scales, zeros, x, ids, out, slots, x_div, experts,
-                  static_cast<int>(outputs), static_cast<int>(inputs), group, 1, 0, gelu, out_f32};
+  if (!records || !x || !ids || !out) return STK_ERR_NULL_POINTER;
+  if ((reinterpret_cast<uintptr_t>(records) | reinterpret_cast<uintptr_t>(x)) % 16) return STK_ERR_BAD_LAYOUT;
+  stk::Int4Args a{static_cast<const unsigned char*>(records), x, ids, out, 0, 0, x_div, experts,
+                  static_cast<int>(outputs), static_cast<int>(inputs), 0, gelu, out_f32};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == STK_BF16 ? stk::int4_launch<__nv_bfloat16>(a, s) : stk::int4_launch<__half>(a, s);
+  return dtype == STK_BF16 ? stk::int4_by_group<__nv_bfloat16>(a, group, zeros, slots, s)
+                           : stk::int4_by_group<__half>(a, group, zeros, slots, s);
 }
 
 extern "C" int stk_b200_int4_combine(const float* y, const int32_t* ids, const float* weights, void* out, int64_t tokens,

@@ -11,37 +11,51 @@ import torch
 from stk_b200.backend import lib as _lib
 
 GROUPS = (32, 64, 128)
+MAX_EXPERTS = 1024
+MAX_GROUPS = 512       # of the inputs
+# Where in a 16-bit float with the exponent of 16 the step is 1: the first bit of a code (int4_sm100.cuh).
+_BITS = {torch.float16: 6, torch.bfloat16: 3}
+
+
+def _turn(words, bits):
+    """The int32 words turned left by `bits`."""
+    return (words << bits) | ((words >> (32 - bits)) & ((1 << bits) - 1))
 
 
 class Int4Experts:
-    """The 4-bit weights [num_experts, outputs, inputs] of a set of experts in the kernels' layout (pack_int4)."""
+    """The 4-bit weights [num_experts, outputs, inputs] of a set of experts in the kernels' layout (pack_int4): records of
+    32 outputs x 128 inputs, each with its codes, scales and zero points."""
 
-    __slots__ = ("words", "scales", "zeros", "num_experts", "outputs", "inputs", "group", "dtype")
+    __slots__ = ("records", "num_experts", "outputs", "inputs", "group", "zero_points", "dtype")
 
-    def __init__(self, words, scales, zeros, num_experts, outputs, inputs, group):
-        self.words, self.scales, self.zeros, self.dtype = words, scales, zeros, scales.dtype
+    def __init__(self, records, num_experts, outputs, inputs, group, zero_points, dtype):
+        self.records, self.dtype, self.zero_points = records, dtype, zero_points
         self.num_experts, self.outputs, self.inputs, self.group = num_experts, outputs, inputs, group
 
     @property
     def device(self):
-        return self.words.device
+        return self.records.device
 
     def to(self, device):
-        move = lambda t: None if t is None else t.to(device)
-        return Int4Experts(move(self.words), move(self.scales), move(self.zeros), self.num_experts, self.outputs,
-                           self.inputs, self.group)
+        return Int4Experts(self.records.to(device), self.num_experts, self.outputs, self.inputs, self.group,
+                           self.zero_points, self.dtype)
 
     def dequantize(self, dtype=torch.float32):
         """The weights as numbers, [num_experts, outputs, inputs]."""
-        e, strips, chunks = self.words.shape[:3]
-        b = self.words.view(e, strips, chunks, 8, 4, 2, 2, 2, 2)                  # g, t, h, s, b, p
-        codes = torch.stack((b & 15, b >> 4), dim=-1)                             # ..., r
-        codes = codes.permute(0, 1, 9, 3, 2, 5, 4, 6, 8, 7)                       # strip r g, chunk h t s p b
-        codes = codes.reshape(e, strips * 16, chunks * 64)[:, :self.outputs, :self.inputs].to(dtype)
-        per_row = lambda t: t.transpose(2, 3).reshape(e, strips * 16, -1)[:, :self.outputs].to(dtype)
-        zero = 8 if self.zeros is None else per_row(self.zeros)[..., None]
-        codes = codes.reshape(e, self.outputs, -1, self.group) - zero
-        return (codes * per_row(self.scales)[..., None]).reshape(e, self.outputs, self.inputs)
+        records = self.records
+        e, blocks, units, _ = records.shape
+        n = 128 // self.group                           # groups of a record
+        words = _turn(records[..., :2048].contiguous().view(torch.int32), 32 - _BITS[self.dtype])
+        b = words.view(torch.uint8).view(e, blocks, units, 2, 2, 8, 4, 2, 2, 2, 2)  # strip, half, g, t, h, s, b, p
+        codes = torch.stack((b & 15, b >> 4), dim=-1)                               # ..., r
+        codes = codes.permute(0, 1, 3, 11, 5, 2, 4, 7, 6, 8, 10, 9)                 # strip r g, unit half h t s p b
+        codes = codes.reshape(e, blocks * 32, units * n, self.group).to(dtype)
+        per_row = lambda t: t.view(e, blocks, units, n, 2, 8, 2).permute(0, 1, 4, 6, 5, 2, 3).reshape(
+            e, blocks * 32, units * n, 1).to(dtype)    # strip r g, unit group
+        zero = per_row(records[..., 2048 + 64 * n:].contiguous()) if self.zero_points else 8
+        scales = per_row(records[..., 2048:2048 + 64 * n].contiguous().view(self.dtype))
+        whole = ((codes - zero) * scales).view(e, blocks * 32, units * 128)
+        return whole[:, :self.outputs, :self.inputs].contiguous()
 
 
 def pack_int4(codes, scales, zeros=None):
@@ -54,12 +68,14 @@ def pack_int4(codes, scales, zeros=None):
         raise ValueError(f"pack_int4: codes must be uint8 [experts, outputs, inputs / 2], got {codes.dtype} "
                          f"{tuple(codes.shape)}")
     experts, outputs, inputs = codes.shape[0], codes.shape[1], 2 * codes.shape[2]
-    if min(experts, outputs, inputs) < 1:
-        raise ValueError(f"pack_int4: empty weights {tuple(codes.shape)}")
+    if min(experts, outputs, inputs) < 1 or experts > MAX_EXPERTS:
+        raise ValueError(f"pack_int4: 1 to {MAX_EXPERTS} experts with weights, got {tuple(codes.shape)}")
     if scales.dim() != 3 or tuple(scales.shape[:2]) != (experts, outputs) or scales.shape[2] < 1 \
             or inputs % scales.shape[2] or inputs // scales.shape[2] not in GROUPS:
         raise ValueError(f"pack_int4: scales must be [{experts}, {outputs}, {inputs} / group] with a group of "
                          f"{', '.join(map(str, GROUPS))} inputs, got {tuple(scales.shape)}")
+    if scales.shape[2] > MAX_GROUPS:
+        raise ValueError(f"pack_int4: at most {MAX_GROUPS} groups of inputs, got {scales.shape[2]}")
     if scales.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"pack_int4: scales are float16 or bfloat16, got {scales.dtype}")
     if zeros is not None and (zeros.dtype != torch.uint8 or zeros.shape != scales.shape):
@@ -68,17 +84,25 @@ def pack_int4(codes, scales, zeros=None):
         raise ValueError("pack_int4: codes, scales and zeros must be on one device")
     if zeros is not None and bool((zeros > 15).any()):
         raise ValueError("pack_int4: zero points are 0..15")
-    group, strips, chunks = inputs // scales.shape[2], (outputs + 15) // 16, (inputs + 63) // 64
-    pad = (0, 32 * chunks - inputs // 2, 0, 16 * strips - outputs)
-    words = torch.empty((experts, strips, chunks, 32, 16), dtype=torch.uint8, device=codes.device)
+    group, blocks, units = inputs // scales.shape[2], (outputs + 31) // 32, (inputs + 127) // 128
+    n = 128 // group                                    # groups of a record
+    size = _lib.load().stk_b200_int4_record_bytes(group, int(zeros is not None))
+    records = torch.empty((experts, blocks, units, size), dtype=torch.uint8, device=codes.device)
+    pad = torch.nn.functional.pad
+    more = 32 * blocks - outputs
     for e in range(experts):                           # (one at a time: no second copy of all weights)
-        v = torch.nn.functional.pad(codes[e], pad).view(strips, 2, 8, chunks, 2, 4, 2, 2)  # r, g, chunk, h, t, s, p
-        lo, hi = v[:, 0], v[:, 1]                      # rows g and g + 8
+        v = pad(codes[e], (0, 64 * units - inputs // 2, 0, more)).view(blocks, 2, 2, 8, units, 2, 2, 4, 2, 2)
+        lo, hi = v[:, :, 0], v[:, :, 1]                 # rows g and g + 8: strip, g, unit, half, h, t, s, p
         b = torch.stack(((lo & 15) | (hi << 4), (lo >> 4) | (hi & 0xF0)), dim=-2)          # ..., s, b, p
-        words[e] = b.permute(0, 2, 1, 4, 3, 5, 6, 7).reshape(strips, chunks, 32, 16)       # chunk, g, t, h, s, b, p
-    by_strip = lambda t: torch.nn.functional.pad(t, (0, 0, 0, 16 * strips - outputs)).view(
-        experts, strips, 16, -1).transpose(2, 3).contiguous()
-    return Int4Experts(words, by_strip(scales), None if zeros is None else by_strip(zeros), experts, outputs, inputs, group)
+        b = b.permute(0, 3, 1, 4, 2, 6, 5, 7, 8, 9).reshape(blocks, units, 2048)           # unit, strip, half, g, t, h, s, b, p
+        one = records[e]
+        one[..., :2048] = _turn(b.view(torch.int32), _BITS[scales.dtype]).view(torch.uint8)
+        per_row = lambda t: pad(t[e], (0, n * units - t.shape[2], 0, more)).view(blocks, 2, 2, 8, units, n).permute(
+            0, 4, 5, 1, 3, 2).reshape(blocks, units, 32 * n)  # unit, group, strip, g, r
+        one[..., 2048:2048 + 64 * n] = per_row(scales).view(torch.uint8)
+        if zeros is not None:
+            one[..., 2048 + 64 * n:] = per_row(zeros)
+    return Int4Experts(records, experts, outputs, inputs, group, zeros is not None, scales.dtype)
 
 
 def quantize_int4(w, group=128, zero_points=False):
@@ -135,9 +159,9 @@ def _check_call(what, x, w, expert_ids):
 def _matvec(x, w, ids, x_div, gelu, out):
     with _lib.on_device(x.device):
         rc = _lib.load().stk_b200_int4_matvec(
-            _lib.ptr(w.words), _lib.ptr(w.scales), _lib.ptr(w.zeros), _lib.ptr(x), _lib.ptr(ids), _lib.ptr(out),
-            ids.numel(), x_div, w.num_experts, w.outputs, w.inputs, w.group, int(gelu),
-            int(out.dtype == torch.float32), _lib.dtype_code(w.dtype), _lib.stream_ptr(x.device))
+            _lib.ptr(w.records), _lib.ptr(x), _lib.ptr(ids), _lib.ptr(out), ids.numel(), x_div, w.num_experts, w.outputs,
+            w.inputs, w.group, int(w.zero_points), int(gelu), int(out.dtype == torch.float32), _lib.dtype_code(w.dtype),
+            _lib.stream_ptr(x.device))
     _lib.check(rc, "stk_b200_int4_matvec")
     return out
 

@@ -62,6 +62,30 @@ def test_the_same_expert_for_every_choice_and_for_none():
     check_matvec(40, 2, 3, 40, 128, 64, torch.float16, True, ids=torch.full((40, 2), -1))
 
 
+@pytest.mark.parametrize("tokens,experts,outputs,inputs,group,zeros", [
+    (6, 8, 14336, 2176, 128, False), (20, 4, 9000, 4096, 64, True), (24, 3, 5000, 1120, 32, True), (160, 2, 2000, 640, 64, False)])
+def test_shares_of_many_rows(tokens, experts, outputs, inputs, group, zeros):
+    """Enough rows that a block takes them in groups of every size, and changes experts on its way; more slots than one
+    launch takes.  Against 64 bits on the GPU."""
+    from stk_b200 import dmoe
+    dtype = torch.bfloat16
+    g = torch.Generator(device="cuda").manual_seed(outputs)
+    packed = torch.randint(0, 256, (experts, outputs, inputs // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scales = (0.01 + 0.02 * torch.rand(experts, outputs, inputs // group, generator=g, device="cuda")).to(dtype)
+    zero = torch.randint(0, 16, scales.shape, generator=g, device="cuda", dtype=torch.uint8) if zeros else None
+    w = dmoe.pack_int4(packed, scales, zero)
+    x = torch.randn(tokens, inputs, generator=g, device="cuda").to(dtype)
+    ids = torch.randint(0, experts, (tokens, 2), generator=g, device="cuda")
+    y = dmoe.int4_matvec(x, w, ids)
+    for e in range(experts):
+        full = w.dequantize(torch.float32)[e].double()
+        token, choice = torch.nonzero(ids == e, as_tuple=True)
+        expect, size = x[token].double() @ full.t(), x[token].double().abs() @ full.abs().t()
+        tol = half_step(dtype) * expect.abs() + ((inputs / 32 + 16) * U32 + 2.0 ** -22) * size
+        assert bool(((y[token, choice].double() - expect).abs() <= tol).all())
+    assert torch.equal(y, dmoe.int4_matvec(x, w, ids))
+
+
 def test_one_matrix_views_and_streams():
     from stk_b200 import dmoe
     codes, packed, scales, zero = bits(1, 50, 128, 64, torch.bfloat16, True)

@@ -30,19 +30,26 @@ def test_pack_and_back(experts, outputs, inputs, group, zeros):
     assert torch.equal(w.dequantize(torch.float64), values(codes, scales, zero, group))
 
 
-def test_layout_of_one_word():
-    """The documented place of a weight: strip, chunk, lane (g, t), word 2h + s, nibble 4b + 2p + r."""
+def test_layout_of_one_record():
+    """The documented place of a weight: strip, half, lane (g, t), word 2h + s, nibble 4b + 2p + r; and of its scale and
+    zero point: group, strip, g, r."""
     from stk_b200 import dmoe
-    for row, col in ((0, 0), (5, 1), (8, 2), (23, 63), (31, 127), (17, 100)):
-        codes = torch.zeros(1, 32, 128, dtype=torch.uint8)
+    for row, col in ((0, 0), (5, 1), (8, 2), (23, 63), (31, 127), (17, 100), (40, 190)):
+        codes = torch.zeros(1, 64, 256, dtype=torch.uint8)
         codes[0, row, col] = 15
-        w = dmoe.pack_int4(codes[..., 0::2] | (codes[..., 1::2] << 4), torch.ones(1, 32, 4, dtype=torch.float16))
-        r, g = row % 16 // 8, row % 8
+        scales, zeros = torch.zeros(1, 64, 4, dtype=torch.float16), torch.zeros(1, 64, 4, dtype=torch.uint8)
+        scales[0, row, col // 64], zeros[0, row, col // 64] = 1.0, 7
+        w = dmoe.pack_int4(codes[..., 0::2] | (codes[..., 1::2] << 4), scales, zeros)
+        assert w.records.shape == (1, 2, 2, 2048 + 128 + 64) and int((w.records != 0).sum()) in (3, 4)
+        record = w.records[0, row // 32, col // 128].clone()
+        strip, r, g, half = row % 32 // 16, row % 16 // 8, row % 8, col % 128 // 64
         h, t, s, p, b = col % 64 // 32, col % 32 // 8, col % 8 // 4, col % 4 // 2, col % 2
-        words = w.words.view(1, 2, 2, 32, 16).contiguous().view(torch.int32)
-        expect = 15 << 4 * (4 * b + 2 * p + r)
-        assert int(words[0, row // 16, col // 64, 4 * g + t, 2 * h + s]) & 0xffffffff == expect
-        assert int((words != 0).sum()) == 1
+        expect = 15 << 4 * (4 * b + 2 * p + r)            # turned left by 6 bits for float16
+        expect = (expect << 6 | expect >> 26) & 0xffffffff
+        words = record[:2048].view(torch.int32).view(2, 2, 32, 4)
+        assert int(words[strip, half, 4 * g + t, 2 * h + s]) & 0xffffffff == expect
+        assert float(record[2048:2176].view(torch.float16).view(2, 2, 8, 2)[half, strip, g, r]) == 1.0
+        assert int(record[2176:].view(2, 2, 8, 2)[half, strip, g, r]) == 7
 
 
 @pytest.mark.parametrize("zero_points", [False, True])
@@ -57,7 +64,9 @@ def test_quantize_is_within_half_a_step(zero_points, dtype):
     w[0, :64, 5] = 0.0                                    # a group of zeros stays one
     q = dmoe.quantize_int4(w, group=64, zero_points=zero_points)
     back = q.dequantize(torch.float64)
-    scales = q.scales.transpose(2, 3).reshape(2, 48, 4).double().repeat_interleave(64, 2)
+    v = w.double().transpose(1, 2).reshape(2, 48, 4, 64)
+    step = (v.amax(3).clamp(min=0) - v.amin(3).clamp(max=0)) / 15 if zero_points else v.abs().amax(3) / 7
+    scales = step.to(dtype).double().repeat_interleave(64, 2)
     bound = (0.5 + (0.5 if zero_points else 0) + 16 * torch.finfo(dtype).eps / 2) * scales
     assert bool(((back - w.double().transpose(1, 2)).abs() <= bound).all())
     assert not bool(back[0, 5, :64].any())
@@ -70,7 +79,9 @@ def test_refusals():
                 lambda: dmoe.pack_int4(packed, scales.float()), lambda: dmoe.pack_int4(packed, scales[:, :8]),
                 lambda: dmoe.pack_int4(packed, scales[:, :, :0]), lambda: dmoe.pack_int4(packed, scales.repeat(1, 1, 4)),
                 lambda: dmoe.pack_int4(packed, scales, zero.int()), lambda: dmoe.pack_int4(packed, scales, zero[:1]),
-                lambda: dmoe.pack_int4(packed, scales, zero + 16), lambda: dmoe.pack_int4(packed[:0], scales[:0]),
+                lambda: dmoe.pack_int4(packed, scales, zero + 16),
+                lambda: dmoe.pack_int4(torch.zeros(1, 1, 513 * 16, dtype=torch.uint8), torch.ones(1, 1, 513).half()),
+                lambda: dmoe.pack_int4(packed[:0], scales[:0]),
                 lambda: dmoe.quantize_int4(torch.randn(2, 64, 8)), lambda: dmoe.quantize_int4(torch.randn(64, 8).half()),
                 lambda: dmoe.quantize_int4(torch.randn(2, 96, 8).half()),
                 lambda: dmoe.quantize_int4(torch.randn(2, 64, 8).half(), group=16)):
@@ -92,10 +103,12 @@ def test_entry_points_check_before_any_launch():
     L = lib.load()
     p = 4096                                              # an aligned address that is never read
     call = lambda slots=4, div=2, experts=2, n=16, k=128, group=64, dtype=1, x=p, words=p: L.stk_b200_int4_matvec(
-        words, p, None, x, p, p, slots, div, experts, n, k, group, 0, 0, dtype, None)
+        words, x, p, p, slots, div, experts, n, k, group, 0, 0, 0, dtype, None)
+    assert [L.stk_b200_int4_record_bytes(g, z) for g in (16, 32, 64, 128) for z in (0, 1)] == [
+        0, 0, 2304, 2432, 2176, 2240, 2112, 2144]
     assert call(slots=0) == 0 and call(slots=-1) == -2 and call(div=0) == -2 and call(experts=0) == -2 and call(n=0) == -2
     assert call(k=96) == -2 and call(group=16) == -2 and call(dtype=3) == -3 and call(dtype=2) == -3
-    assert call(experts=70000) == -9 and call(x=None) == -1 and call(x=p + 2) == -4 and call(words=p + 8) == -4
+    assert call(k=513 * 64) == -9 and call(experts=70000) == -9 and call(x=None) == -1 and call(x=p + 2) == -4 and call(words=p + 8) == -4
     assert L.stk_b200_int4_combine(p, p, p, None, 4, 2, 2, 16, 1, None) == -1
     assert L.stk_b200_int4_combine(p, p, p, p, 4, 0, 2, 16, 1, None) == -2
     assert L.stk_b200_int4_combine(p, p, p, p, 4, 2, 2, 16, 3, None) == -3
