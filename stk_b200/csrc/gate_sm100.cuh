@@ -10,9 +10,9 @@
 // Everything is computed in 32 bits; the only rounding to fewer is that of the logits' gradient to their type.
 //
 // Choices are made on the logits themselves (both scores are monotone), by exact comparison: equal logits go to
-// the lower expert, -0 equals +0, a NaN counts as the largest value there is (its weights come out as NaN), and
-// -inf is never chosen: where fewer than k logits are left, and in rows that the token mask switches off, the
-// remaining choices are -1 with weight 0.
+// the lower expert, -0 equals +0, a NaN counts as +inf (and makes the row's weights NaN), and -inf is never chosen:
+// where fewer than k logits are left, and in rows that the token mask switches off, the remaining choices are -1 with
+// weight 0.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -32,23 +32,78 @@ template <> __device__ __forceinline__ float from_f32<float>(float v) { return v
 template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// N consecutive elements moved by one access.
+// N consecutive elements, moved by one access of 2 to 16 bytes and held as the words of that access: elements of 16 bits
+// in registers of their own, where an access is conditional, are taken apart and put together again one by one (117
+// against 79 us for the sum of 2 x 32768 rows of 2048).
+template <int kBytes> struct RawOf;
+template <> struct RawOf<2> { using Type = unsigned short; };
+template <> struct RawOf<4> { using Type = unsigned int; };
+template <> struct RawOf<8> { using Type = uint2; };
+template <> struct RawOf<16> { using Type = uint4; };
+template <typename T, int N> using Raw = typename RawOf<sizeof(T) * N>::Type;
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
-  T v[N];
+__device__ __forceinline__ Raw<T, N> load_raw(const T* from) {
+  return __ldcs(reinterpret_cast<const Raw<T, N>*>(from));  // read once
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_raw(T* to, const Raw<T, N>& v) {
+  *reinterpret_cast<Raw<T, N>*>(to) = v;
+}
+template <typename T, int N>
+__device__ __forceinline__ void stream_raw(T* to, const Raw<T, N>& v) {
+  __stcs(reinterpret_cast<Raw<T, N>*>(to), v);
+}
+template <typename T> struct Two;  // of the 16-bit types
+template <> struct Two<__half> {
+  __device__ static float2 to(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+  __device__ static uint32_t from(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
-
-// Order-preserving image of a float: larger value, larger key.  0 is below every value.
-__device__ __forceinline__ uint32_t order_key(float f) {
-  f += 0.0f;  // -0 becomes +0
-  if (f != f) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(f);
-  return b ^ (static_cast<uint32_t>(static_cast<int32_t>(b) >> 31) | 0x80000000u);
+template <> struct Two<__nv_bfloat16> {
+  __device__ static float2 to(uint32_t w) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w)); }
+  __device__ static uint32_t from(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Raw<T, N>& v, float (&f)[N]) {
+  if constexpr (sizeof(T) * N == 2) {
+    f[0] = to_f32(*reinterpret_cast<const T*>(&v));
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&v);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) f[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) {
+        const float2 t = Two<T>::to(w[i]);
+        f[2 * i] = t.x;
+        f[2 * i + 1] = t.y;
+      }
+    }
+  }
 }
-__device__ __forceinline__ float order_value(uint32_t key) {
-  return __uint_as_float((key & 0x80000000u) ? key ^ 0x80000000u : ~key);
+template <typename T, int N>
+__device__ __forceinline__ Raw<T, N> pack(const float (&f)[N]) {
+  Raw<T, N> v;
+  if constexpr (sizeof(T) * N == 2) {
+    *reinterpret_cast<T*>(&v) = from_f32<T>(f[0]);
+  } else {
+    uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] = __float_as_uint(f[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i) w[i] = Two<T>::from(f[2 * i], f[2 * i + 1]);
+    }
+  }
+  return v;
 }
-constexpr uint32_t kKeyNegInf = 0x007fffffu;
 
 __device__ __forceinline__ float log_sigmoid(float l) { return fminf(l, 0.0f) - log1pf(expf(-fabsf(l))); }
 __device__ __forceinline__ float sigmoid(float l) { return 1.0f / (1.0f + expf(-l)); }
@@ -66,30 +121,37 @@ __device__ __forceinline__ void gate_load(const T* row, int experts, int lane, f
   for (int c = 0; c < V / N; ++c) {
     const int at = (c * G + lane) * N;
     if (kVec) {
-      Pack<T, N> p;
-      if (at < experts) p = *reinterpret_cast<const Pack<T, N>*>(row + at);
+      Raw<T, N> raw;
+      if (at < experts) raw = load_raw<T, N>(row + at);
+      float f[N];
+      unpack<T, N>(raw, f);
 #pragma unroll
-      for (int j = 0; j < N; ++j) val[c * N + j] = at < experts ? to_f32(p.v[j]) : -INFINITY;
+      for (int j = 0; j < N; ++j) val[c * N + j] = at < experts ? f[j] : -INFINITY;
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j) val[c * N + j] = at + j < experts ? to_f32(row[at + j]) : -INFINITY;
     }
   }
 }
-template <typename T, int G, int V>
-__device__ __forceinline__ int gate_index(int v, int lane) {
-  constexpr int N = V < 16 / static_cast<int>(sizeof(T)) ? V : 16 / static_cast<int>(sizeof(T));
-  return ((v / N) * G + lane) * N + v % N;
+// exp(d) for d <= 0 as 2^(d log2(e)): 2^-22 and |d| 2^-24 off, relative.  (Differences are taken first: the product of the
+// type's lowest value would overflow.)
+__device__ __forceinline__ float gate_exp(float d) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d * 1.44269504f));
+  return r;
 }
 
 // G lanes per token, V logits per lane.  k rounds, each finding the largest remaining (value, lowest index) in
-// the lane's registers and then across the lanes by butterfly shuffles; a bit per register remembers what is gone.
-// stats (optional): the row's maximum and 1 / sum, for the backward pass of the plain softmax.
+// the lane's registers and then across the lanes by butterfly shuffles; what is chosen becomes -inf.
+// stats (optional): the row's maximum and sum, for the backward pass of the plain softmax.
+// Bound by its arithmetic (about 250 instructions a lane for 64 experts, 2 choices); few lanes with many logits each,
+// since a shuffle step costs as much as three logits.
 template <typename T, int G, int V, bool kVec>
 __global__ void __launch_bounds__(kGateThreads)
 gate_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int experts, int k, int sigmoid_score,
             int normalize, const uint8_t* __restrict__ mask, float* __restrict__ weights,
             int32_t* __restrict__ ids, float2* __restrict__ stats) {
+  constexpr int N = V < 16 / static_cast<int>(sizeof(T)) ? V : 16 / static_cast<int>(sizeof(T));
   extern __shared__ float chosen_all[];  // [kGateThreads / G][k]
   const int group = threadIdx.x / G, lane = threadIdx.x % G;
   float* chosen = chosen_all + group * k;
@@ -103,54 +165,62 @@ gate_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int expert
 #pragma unroll
     for (int v = 0; v < V; ++v) val[v] = -INFINITY;
   }
-  uint32_t key[V];
+  float nan = 0.0f;                      // NaN if a logit is one
+  float check = 0.0f;
 #pragma unroll
-  for (int v = 0; v < V; ++v) key[v] = gate_index<T, G, V>(v, lane) < experts ? order_key(val[v]) : 0u;
+  for (int v = 0; v < V; ++v) check += val[v];
+  if (check != check) {                  // a NaN, or infinities of both signs
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      if (val[v] != val[v]) {
+        nan = val[v];
+        val[v] = INFINITY;
+      }
+  }
+#pragma unroll
+  for (int off = G / 2; off > 0; off >>= 1) nan += __shfl_xor_sync(0xffffffffu, nan, off);
 
-  uint32_t gone = 0;
-  float top = -INFINITY, sum = 0.0f;  // the maximum; the denominator
+  const bool plain_softmax = !sigmoid_score && !normalize;
+  float top = 0.0f, sum = 0.0f;  // the maximum, the denominator
   for (int j = 0; j < k; ++j) {
-    uint32_t best = 0;
+    float best = -INFINITY;
     int at = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const uint32_t c = (gone >> v) & 1u ? 0u : key[v];
-      if (c > best) {
-        best = c;
-        at = v;
-      }
+      at = val[v] > best ? v : at;
+      best = fmaxf(best, val[v]);
     }
-    int index = gate_index<T, G, V>(0, lane);
-#pragma unroll
-    for (int v = 1; v < V; ++v) index = at == v ? gate_index<T, G, V>(v, lane) : index;
-    const int mine = index;
-    const uint32_t my_best = best;
+    const int mine = (at / N * G + lane) * N + at % N;
+    int index = mine;
 #pragma unroll
     for (int off = G / 2; off > 0; off >>= 1) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, best, off);
+      const float other = __shfl_xor_sync(0xffffffffu, best, off);
       const int other_index = __shfl_xor_sync(0xffffffffu, index, off);
       if (other > best || (other == best && other_index < index)) {
         best = other;
         index = other_index;
       }
     }
-    if (my_best == best && mine == index) gone |= 1u << at;
-    const bool taken = best > kKeyNegInf;
-    const float l = order_value(best);
+    const bool taken = best > -INFINITY;
     if (j == 0) {
-      top = taken ? l : -INFINITY;
-      if (!sigmoid_score && !normalize) {
+      top = taken ? best : 0.0f;
+      if (plain_softmax) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) sum += taken ? expf(val[v] - top) : 0.0f;
+        for (int v = 0; v < V; ++v) sum += gate_exp(val[v] - top);
 #pragma unroll
         for (int off = G / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
       }
       if (sigmoid_score && normalize) top = log_sigmoid(top);
     }
+    if (j + 1 < k) {
+      const int gone = mine == index ? at : -1;
+#pragma unroll
+      for (int v = 0; v < V; ++v) val[v] = v == gone ? -INFINITY : val[v];
+    }
     float w = 0.0f;
     if (taken) {
-      if (!sigmoid_score) w = expf(l - top);
-      else w = normalize ? expf(log_sigmoid(l) - top) : sigmoid(l);
+      if (!sigmoid_score) w = gate_exp(best - top);
+      else w = normalize ? expf(log_sigmoid(best) - top) : sigmoid(best);
       if (normalize) sum += w;
     }
     if (lane == 0 && here) {
@@ -161,7 +231,7 @@ gate_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int expert
   __syncwarp();
   if (!here) return;
   if (sigmoid_score && !normalize) sum = 1.0f;
-  for (int j = lane; j < k; j += G) weights[t * k + j] = sum != 0.0f ? chosen[j] / sum : 0.0f;
+  for (int j = lane; j < k; j += G) weights[t * k + j] = sum != 0.0f ? chosen[j] / sum + nan : 0.0f;
   if (lane == 0 && stats != nullptr) stats[t] = make_float2(top, sum);
 }
 
@@ -191,7 +261,7 @@ gate_backward_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, i
     gate_load<T, G, V, kVec>(logits + t * ld, experts, lane, val);
     const float scale = -inner / s.y;
 #pragma unroll
-    for (int v = 0; v < V; ++v) val[v] = scale * expf(val[v] - s.x);
+    for (int v = 0; v < V; ++v) val[v] = scale * gate_exp(val[v] - s.x);
   } else {
 #pragma unroll
     for (int v = 0; v < V; ++v) val[v] = 0.0f;
@@ -216,10 +286,10 @@ gate_backward_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, i
   for (int c = 0; c < V / N; ++c) {
     const int at = (c * G + lane) * N;
     if (kVec) {
-      Pack<T, N> p;
+      float f[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) p.v[j] = from_f32<T>(val[c * N + j]);
-      if (at < experts) *reinterpret_cast<Pack<T, N>*>(out + at) = p;
+      for (int j = 0; j < N; ++j) f[j] = val[c * N + j];
+      if (at < experts) store_raw<T, N>(out + at, pack<T, N>(f));
     } else {
 #pragma unroll
       for (int j = 0; j < N; ++j)
@@ -274,11 +344,11 @@ static int gate_by_alignment(const GateArgs& a) {
 template <typename T>
 static int gate_by_experts(const GateArgs& a) {
   if (a.experts <= 8) return gate_by_alignment<T, 1, 8>(a);
-  if (a.experts <= 16) return gate_by_alignment<T, 2, 8>(a);
-  if (a.experts <= 32) return gate_by_alignment<T, 4, 8>(a);
-  if (a.experts <= 64) return gate_by_alignment<T, 8, 8>(a);
-  if (a.experts <= 128) return gate_by_alignment<T, 16, 8>(a);
-  if (a.experts <= 256) return gate_by_alignment<T, 32, 8>(a);
+  if (a.experts <= 16) return gate_by_alignment<T, 1, 16>(a);
+  if (a.experts <= 32) return gate_by_alignment<T, 2, 16>(a);
+  if (a.experts <= 64) return gate_by_alignment<T, 4, 16>(a);
+  if (a.experts <= 128) return gate_by_alignment<T, 8, 16>(a);
+  if (a.experts <= 256) return gate_by_alignment<T, 16, 16>(a);
   if (a.experts <= 512) return gate_by_alignment<T, 32, 16>(a);
   return gate_by_alignment<T, 32, 32>(a);
 }

@@ -172,14 +172,11 @@ constexpr int kPadRows = 4;                                // rows that a warp l
 template <typename T, int N>
 __device__ __forceinline__ void zero_padding(T* __restrict__ dst, const int32_t* __restrict__ index, int64_t rows,
                                              int64_t hidden, int64_t w, int lane) {
-  Pack<T, N> zero;
-#pragma unroll
-  for (int i = 0; i < N; ++i) zero.v[i] = from_f32<T>(0.0f);
+  const Raw<T, N> zero{};
   const int64_t r0 = w * kPadRows;
   for (int i = 0; i < kPadRows && r0 + i < rows; ++i) {
     if (index[r0 + i] >= 0) continue;
-    Pack<T, N>* out = reinterpret_cast<Pack<T, N>*>(dst + (r0 + i) * hidden);
-    for (int64_t v = lane; v < hidden / N; v += 32) out[v] = zero;
+    for (int64_t v = lane; v < hidden / N; v += 32) store_raw<T, N>(dst + (r0 + i) * hidden + v * N, zero);
   }
 }
 
@@ -197,73 +194,84 @@ sort_rows_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ rows, cons
   const int64_t t = unit / parts;
   if (t >= tokens) return;
   const int64_t vecs = hidden / N, v0 = (unit - t * parts) * kPartVecs + lane;
-  const Pack<T, N>* in = reinterpret_cast<const Pack<T, N>*>(x + t * ld);
-  Pack<T, N> part[kLaneVecs];
+  Raw<T, N> part[kLaneVecs];
 #pragma unroll
   for (int i = 0; i < kLaneVecs; ++i)
-    if (v0 + 32 * i < vecs) part[i] = in[v0 + 32 * i];
+    if (v0 + 32 * i < vecs) part[i] = load_raw<T, N>(x + t * ld + (v0 + 32 * i) * N);
   for (int j = 0; j < k; ++j) {
     const int64_t r = position[t * k + j];
     if (r < 0) continue;
-    Pack<T, N>* out = reinterpret_cast<Pack<T, N>*>(rows + r * hidden);
 #pragma unroll
     for (int i = 0; i < kLaneVecs; ++i)
-      if (v0 + 32 * i < vecs) out[v0 + 32 * i] = part[i];
+      if (v0 + 32 * i < vecs) store_raw<T, N>(rows + r * hidden + (v0 + 32 * i) * N, part[i]);
   }
 }
 
-// out[t] = sum_j weights[t*k+j] * rows[position[t*k+j]] (weights NULL: all ones), in 32 bits, rounded once.
-template <typename T, int N>
+// out[t] = sum_j weights[t*k+j] * rows[position[t*k+j]] (weights NULL: all ones), in 32 bits, rounded once.  A warp takes
+// kSumVecs * 32 vectors of a token; K choices are read at once (K * kSumVecs accesses in flight a lane), so that a token's
+// rows are waited for once and not one after the other.  2 vectors of 16 bytes (2 x 32768 rows of 2048 bf16: 70 us, 4
+// vectors 80, 1 vector 78), 4 narrower ones (4 x 5003 rows of 1001 fp32: 22 us, 2 vectors 29).
+template <typename T, int N> constexpr int kSumVecsOf = sizeof(T) * N == 16 ? 2 : 4;
+template <typename T, int N, int K>
 __global__ void __launch_bounds__(kRowThreads)
 sum_rows_kernel(const T* __restrict__ rows, int64_t ld, const int32_t* __restrict__ position,
                 const float* __restrict__ weights, T* __restrict__ out, int64_t tokens, int k, int64_t hidden, int parts) {
+  constexpr int kSumVecs = kSumVecsOf<T, N>;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t unit = static_cast<int64_t>(blockIdx.x) * kRowWarps + warp;
   const int64_t t = unit / parts;
   if (t >= tokens) return;
-  const int64_t vecs = hidden / N, v0 = (unit - t * parts) * kPartVecs + lane;
-  float acc[kLaneVecs][N];
+  const int64_t vecs = hidden / N, v0 = (unit - t * parts) * (32 * kSumVecs) + lane;
+  float acc[kSumVecs][N];
 #pragma unroll
-  for (int i = 0; i < kLaneVecs; ++i)
+  for (int i = 0; i < kSumVecs; ++i)
 #pragma unroll
     for (int n = 0; n < N; ++n) acc[i][n] = 0.0f;
-#pragma unroll 2
-  for (int j = 0; j < k; ++j) {
-    const int64_t r = position[t * k + j];
-    if (r < 0) continue;
-    const float w = weights != nullptr ? weights[t * k + j] : 1.0f;
-    const Pack<T, N>* in = reinterpret_cast<const Pack<T, N>*>(rows + r * ld);
-    Pack<T, N> part[kLaneVecs];
+  for (int j0 = 0; j0 < k; j0 += K) {
+    int32_t row[K];
+    float w[K];
 #pragma unroll
-    for (int i = 0; i < kLaneVecs; ++i)
-      if (v0 + 32 * i < vecs) part[i] = in[v0 + 32 * i];
+    for (int j = 0; j < K; ++j) {
+      row[j] = j0 + j < k ? position[t * k + j0 + j] : -1;
+      w[j] = j0 + j < k && weights != nullptr ? weights[t * k + j0 + j] : 1.0f;
+    }
+    Raw<T, N> part[K][kSumVecs];
 #pragma unroll
-    for (int i = 0; i < kLaneVecs; ++i)
+    for (int j = 0; j < K; ++j)
 #pragma unroll
-      for (int n = 0; n < N; ++n)
-        if (v0 + 32 * i < vecs) acc[i][n] = fmaf(w, to_f32(part[i].v[n]), acc[i][n]);
+      for (int i = 0; i < kSumVecs; ++i)
+        if (row[j] >= 0 && v0 + 32 * i < vecs)
+          part[j][i] = load_raw<T, N>(rows + row[j] * ld + (v0 + 32 * i) * N);
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+#pragma unroll
+      for (int i = 0; i < kSumVecs; ++i)
+        if (row[j] >= 0 && v0 + 32 * i < vecs) {
+          float f[N];
+          unpack<T, N>(part[j][i], f);
+#pragma unroll
+          for (int n = 0; n < N; ++n) acc[i][n] = fmaf(w[j], f[n], acc[i][n]);
+        }
   }
-  Pack<T, N>* to = reinterpret_cast<Pack<T, N>*>(out + t * hidden);
 #pragma unroll
-  for (int i = 0; i < kLaneVecs; ++i) {
-    Pack<T, N> part;
-#pragma unroll
-    for (int n = 0; n < N; ++n) part.v[n] = from_f32<T>(acc[i][n]);
-    if (v0 + 32 * i < vecs) to[v0 + 32 * i] = part;
-  }
+  for (int i = 0; i < kSumVecs; ++i)
+    if (v0 + 32 * i < vecs) store_raw<T, N>(out + t * hidden + (v0 + 32 * i) * N, pack<T, N>(acc[i]));
 }
 
 // Both gradients of the weighted sum in one pass: dout[t] is read once, every row once, every gradient row is
-// written once.  `warps` warps share a token (dot products joined in shared memory, in order); kDots choices are
-// taken at a time.  drows / dweights may be NULL.
-constexpr int kDots = 8;
-template <typename T, int N>
+// written once.  `warps` warps share a token (dot products joined in shared memory, in order); K choices are taken at a
+// time, kBackVecs vectors of each in flight a lane (2 of 16 bytes, 2 x 16384 rows of 4096 bf16: 121 us, 4 of them 129; 4
+// narrower ones, 4 x 5003 rows of 1001 fp32: 35 us, 2 of them 39).  The gradient rows, larger than what follows can keep
+// in the L2, are stored as streams (129 -> 115 us for 2 x 32768 rows of 2048).  drows / dweights may be NULL.
+template <typename T, int N> constexpr int kBackVecsOf = sizeof(T) * N == 16 ? 2 : 4;
+template <typename T, int N, int K>
 __global__ void __launch_bounds__(kRowThreads)
 unsort_backward_kernel(const T* __restrict__ dout, int64_t ld_dout, const T* __restrict__ rows, int64_t ld_rows,
                        const float* __restrict__ weights, const int32_t* __restrict__ index,
                        const int32_t* __restrict__ position, T* __restrict__ drows, float* __restrict__ dweights,
                        int64_t tokens, int k, int64_t n_rows, int64_t hidden, int warps, int64_t pad_blocks) {
-  __shared__ float dots[kRowWarps][kDots];
+  constexpr int kBackVecs = kBackVecsOf<T, N>;
+  __shared__ float dots[kRowWarps][K];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (blockIdx.x < pad_blocks) {
     zero_padding<T, N>(drows, index, n_rows, hidden, static_cast<int64_t>(blockIdx.x) * kRowWarps + warp, lane);
@@ -273,44 +281,59 @@ unsort_backward_kernel(const T* __restrict__ dout, int64_t ld_dout, const T* __r
   const int part = warp % warps;
   const bool here = t < tokens;
   const int64_t vecs = hidden / N;
-  const Pack<T, N>* grad = reinterpret_cast<const Pack<T, N>*>(dout + t * ld_dout);
-  for (int j0 = 0; j0 < k; j0 += kDots) {
-    float dot[kDots];
+  for (int j0 = 0; j0 < k; j0 += K) {
+    float dot[K], w[K];
+    int32_t row[K];
 #pragma unroll
-    for (int j = 0; j < kDots; ++j) dot[j] = 0.0f;
+    for (int j = 0; j < K; ++j) {
+      const bool there = here && j0 + j < k;
+      dot[j] = 0.0f;
+      row[j] = there ? position[t * k + j0 + j] : -1;
+      w[j] = there && weights != nullptr ? weights[t * k + j0 + j] : 1.0f;
+    }
     if (here) {
-      for (int64_t v = part * 32 + lane; v < vecs; v += warps * 32) {
-        const Pack<T, N> g = grad[v];
+      for (int64_t v0 = part * (32 * kBackVecs) + lane; v0 < vecs; v0 += warps * (32 * kBackVecs)) {
+        Raw<T, N> g[kBackVecs], y[K][kBackVecs];
 #pragma unroll
-        for (int j = 0; j < kDots; ++j) {
-          if (j0 + j >= k) break;
-          const int64_t r = position[t * k + j0 + j];
-          if (r < 0) continue;
-          if (dweights != nullptr) {
-            const Pack<T, N> y = reinterpret_cast<const Pack<T, N>*>(rows + r * ld_rows)[v];
+        for (int i = 0; i < kBackVecs; ++i)
+          if (v0 + 32 * i < vecs) g[i] = load_raw<T, N>(dout + t * ld_dout + (v0 + 32 * i) * N);
+        if (dweights != nullptr) {
 #pragma unroll
-            for (int n = 0; n < N; ++n) dot[j] = fmaf(to_f32(g.v[n]), to_f32(y.v[n]), dot[j]);
-          }
-          if (drows != nullptr) {
-            const float w = weights != nullptr ? weights[t * k + j0 + j] : 1.0f;
-            Pack<T, N> d;
+          for (int j = 0; j < K; ++j)
 #pragma unroll
-            for (int n = 0; n < N; ++n) d.v[n] = from_f32<T>(w * to_f32(g.v[n]));
-            reinterpret_cast<Pack<T, N>*>(drows + r * hidden)[v] = d;
-          }
+            for (int i = 0; i < kBackVecs; ++i)
+              if (row[j] >= 0 && v0 + 32 * i < vecs)
+                y[j][i] = load_raw<T, N>(rows + row[j] * ld_rows + (v0 + 32 * i) * N);
         }
+#pragma unroll
+        for (int j = 0; j < K; ++j)
+#pragma unroll
+          for (int i = 0; i < kBackVecs; ++i) {
+            if (row[j] < 0 || v0 + 32 * i >= vecs) continue;
+            float f[N], other[N];
+            unpack<T, N>(g[i], f);
+            if (drows != nullptr) {
+#pragma unroll
+              for (int n = 0; n < N; ++n) other[n] = w[j] * f[n];
+              stream_raw<T, N>(drows + row[j] * hidden + (v0 + 32 * i) * N, pack<T, N>(other));
+            }
+            if (dweights != nullptr) {
+              unpack<T, N>(y[j][i], other);
+#pragma unroll
+              for (int n = 0; n < N; ++n) dot[j] = fmaf(f[n], other[n], dot[j]);
+            }
+          }
       }
     }
     if (dweights == nullptr) continue;
 #pragma unroll
-    for (int j = 0; j < kDots; ++j) {
-      float d = dot[j];
+    for (int j = 0; j < K; ++j) {
 #pragma unroll
-      for (int off = 16; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
-      if (lane == 0) dots[warp][j] = d;
+      for (int off = 16; off > 0; off >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], off);
+      if (lane == 0) dots[warp][j] = dot[j];
     }
     __syncthreads();
-    if (part == 0 && here && lane < kDots && j0 + lane < k) {
+    if (part == 0 && here && lane < K && j0 + lane < k) {
       float d = 0.0f;
       for (int p = 0; p < warps; ++p) d += dots[warp + p][lane];
       dweights[t * k + j0 + lane] = d;
@@ -373,29 +396,36 @@ enum RowOp { kSortRows, kSumRows, kUnsortBackward };
 template <typename T, int N>
 static int row_launch(RowOp op, const RowArgs& a) {
   const int64_t vecs = a.hidden / N;
-  const int64_t parts = (vecs + kPartVecs - 1) / kPartVecs;
-  const int64_t per_block = kRowWarps;
+  const int part = op == kSumRows ? 32 * kSumVecsOf<T, N> : kPartVecs;
+  const int64_t parts = (vecs + part - 1) / part;
   int64_t pad_blocks = op == kSumRows || a.out == nullptr ? 0 : (a.n_rows + kRowWarps * kPadRows - 1) / (kRowWarps * kPadRows);
   int warps = 1;
-  while (warps < kRowWarps && warps * 64 <= vecs) warps *= 2;
+  while (warps < kRowWarps && warps * 32 * kBackVecsOf<T, N> < vecs) warps *= 2;
   int64_t blocks = op == kUnsortBackward ? (a.tokens + kRowWarps / warps - 1) / (kRowWarps / warps)
-                                         : (a.tokens * parts + per_block - 1) / per_block;
+                                         : (a.tokens * parts + kRowWarps - 1) / kRowWarps;
   blocks += pad_blocks;
   if (blocks > INT32_MAX || parts > INT32_MAX) return STK_ERR_TOO_LARGE;
   if (blocks == 0) return STK_OK;
   const unsigned grid = static_cast<unsigned>(blocks);
   const T* in = static_cast<const T*>(a.a);
   T* out = static_cast<T*>(a.out);
+  const auto sum = [&](auto kernel) {
+    kernel<<<grid, kRowThreads, 0, a.stream>>>(in, a.ld_a, a.position, a.weights, out, a.tokens, a.k, a.hidden,
+                                               static_cast<int>(parts));
+  };
+  const auto backward = [&](auto kernel) {
+    kernel<<<grid, kRowThreads, 0, a.stream>>>(in, a.ld_a, static_cast<const T*>(a.b), a.ld_b, a.weights, a.index,
+                                               a.position, out, a.dweights, a.tokens, a.k, a.n_rows, a.hidden, warps,
+                                               pad_blocks);
+  };
   if (op == kSortRows)
     sort_rows_kernel<T, N><<<grid, kRowThreads, 0, a.stream>>>(in, a.ld_a, out, a.index, a.position, a.tokens, a.k,
                                                                a.n_rows, a.hidden, static_cast<int>(parts), pad_blocks);
   else if (op == kSumRows)
-    sum_rows_kernel<T, N><<<grid, kRowThreads, 0, a.stream>>>(in, a.ld_a, a.position, a.weights, out, a.tokens, a.k,
-                                                              a.hidden, static_cast<int>(parts));
+    a.k == 1 ? sum(sum_rows_kernel<T, N, 1>) : a.k == 2 ? sum(sum_rows_kernel<T, N, 2>) : sum(sum_rows_kernel<T, N, 4>);
   else
-    unsort_backward_kernel<T, N><<<grid, kRowThreads, 0, a.stream>>>(
-        in, a.ld_a, static_cast<const T*>(a.b), a.ld_b, a.weights, a.index, a.position, out, a.dweights, a.tokens, a.k,
-        a.n_rows, a.hidden, warps, pad_blocks);
+    a.k == 1 ? backward(unsort_backward_kernel<T, N, 1>)
+             : a.k == 2 ? backward(unsort_backward_kernel<T, N, 2>) : backward(unsort_backward_kernel<T, N, 4>);
   return cudaGetLastError() == cudaSuccess ? STK_OK : STK_ERR_LAUNCH;
 }
 

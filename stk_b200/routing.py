@@ -87,7 +87,8 @@ class _TopKGate(torch.autograd.Function):
 
 def _host_gate(logits, mask, top_k, score, normalize):
     values = logits.float()
-    ids = torch.sort(values.detach(), dim=1, descending=True, stable=True).indices[:, :top_k]
+    nan = values.detach().isnan()
+    ids = torch.sort(values.detach().masked_fill(nan, torch.inf), dim=1, descending=True, stable=True).indices[:, :top_k]
     top = torch.gather(values, 1, ids)
     valid = top.detach() != -torch.inf
     if mask is not None:
@@ -106,6 +107,7 @@ def _host_gate(logits, mask, top_k, score, normalize):
         weights = torch.softmax(logs, 1)
     else:
         weights = torch.sigmoid(top)
+    weights = weights + torch.zeros(()).masked_fill(nan.any(1, keepdim=True), torch.nan)
     return weights.masked_fill(~valid, 0.0), ids.masked_fill(~valid, -1).to(torch.int32)
 
 
@@ -117,7 +119,7 @@ def top_k_gate(logits, top_k, score="softmax", normalize=True, token_mask=None):
     "sigmoid"; normalize: the k weights of a token are scaled to add up to 1.  Equal logits go to the lower expert, and
     an expert whose logit is -inf is never chosen.  A choice that is left without an expert (fewer than k logits above
     -inf, or token_mask[t] False: bool [T], padding tokens) has id -1 and weight 0 and passes no gradient; plan_tokens
-    gives it no row.  A NaN counts as the largest logit and makes the token's weights NaN."""
+    gives it no row.  A NaN counts as +inf among the logits and makes the token's weights NaN."""
     if logits.dim() != 2:
         raise ValueError(f"top_k_gate: logits must be [tokens, experts], got {tuple(logits.shape)}")
     if score not in _SCORES:
