@@ -415,7 +415,10 @@ int stk_b200_ep_return(const void* result, const int64_t* tags, const uint64_t* 
  *   hold zero points (8 everywhere otherwise).  dtype: of x and the scales; out: the same type or, with
  *   out_f32, float.  gelu: the GeLU of the product.  group 32, 64 or 128; at most 512 groups
  *   of inputs and 1024 experts.
- * int4_combine: out[t] = sum_j weights[slot] * y[slot] over the slots of token t that have an expert.
+ * int4_mlp: out[t] = sum_j weights[slot] * W2_e gelu(W1_e x[t]) over the slots of token t that have an expert, by two
+ *   int4_matvec and a weighted sum.  x [tokens, hidden] and out [tokens, outputs] of `dtype`; records1: ffn outputs,
+ *   hidden inputs; records2: `outputs` outputs, ffn inputs.  workspace: int4_mlp_workspace_bytes(tokens * top_k, ...),
+ *   16-byte aligned, of one call at a time.
  */
 int stk_b200_top_k_gate(const void* logits, int64_t ld, int64_t tokens, int experts, int top_k, int score,
                         int normalize, const uint8_t* token_mask, float* weights, int32_t* ids, float* stats,
@@ -439,8 +442,11 @@ size_t stk_b200_int4_record_bytes(int group, int zeros);
 int stk_b200_int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots, int x_div,
                          int experts, int64_t outputs, int64_t inputs, int group, int zeros, int gelu, int out_f32,
                          int dtype, void* stream);
-int stk_b200_int4_combine(const float* y, const int32_t* ids, const float* weights, void* out, int64_t tokens,
-                          int top_k, int experts, int64_t outputs, int dtype, void* stream);
+size_t stk_b200_int4_mlp_workspace_bytes(int64_t slots, int64_t ffn, int64_t outputs);
+int stk_b200_int4_mlp(const void* records1, const void* records2, const void* x, const int32_t* ids,
+                      const float* weights, void* out, int64_t tokens, int top_k, int experts, int64_t hidden,
+                      int64_t ffn, int64_t outputs, int group1, int zeros1, int group2, int zeros2, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * 32-bit block indices.  The reference stores block row / column indices as int16 and rejects matrices

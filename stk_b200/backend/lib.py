@@ -84,7 +84,9 @@ SIGNATURES = {
     "stk_b200_int4_record_bytes": (_c_size, [_c_int, _c_int]),
     "stk_b200_int4_matvec": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_i64, _c_int,
                                       _c_int, _c_int, _c_int, _c_int, _c_ptr]),
-    "stk_b200_int4_combine": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_int, _c_ptr]),
+    "stk_b200_int4_mlp_workspace_bytes": (_c_size, [_c_i64, _c_i64, _c_i64]),
+    "stk_b200_int4_mlp": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_int, _c_int, _c_i64, _c_i64,
+                                   _c_i64, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr, _c_size, _c_ptr]),
     "stk_b200_ep_return": (_c_int, [_c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i64, _c_int, _c_i64, _c_i64, _c_ptr]),
 }
 # every routine that takes or produces int16 block indices has an _i32 twin with the same signature
@@ -203,6 +205,18 @@ class on_device:
         if self.prev is not None:
             torch.cuda.set_device(self.prev)
         return False
+
+
+def launch(name, device, *args):
+    """Calls the entry point `name` with `args` and the current stream of `device` (a tensor's) and checks its status."""
+    fn, index = getattr(_lib or load(), name), device.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index) or None)
+    else:
+        with on_device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index) or None)
+    if rc:
+        check(rc, name)
 
 
 def entry(name, index_tensor):

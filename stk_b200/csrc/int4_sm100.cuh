@@ -422,6 +422,9 @@ int4_matvec_kernel(const Int4Args a) {
   Smem& sm = *reinterpret_cast<Smem*>(int4_smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int32_t* ids = a.ids + a.first_slot;
+  // The kernel after this one, if it was launched so, sets up and starts its copies while this one runs out; it waits for
+  // this one's results where it first reads x.
+  pdl_launch_dependents();
 
   // the slots, expert by expert, and the (expert, tile) entries of up to 8 * kInt4MaxTiles of them
   for (int e = threadIdx.x; e < a.experts; e += kInt4Threads) sm.counter[e] = 0;
@@ -494,7 +497,10 @@ int4_matvec_kernel(const Int4Args a) {
   const int blocks = (a.outputs + kInt4Rows - 1) / kInt4Rows, units = (a.inputs + kInt4Inputs - 1) / kInt4Inputs;
   const int64_t rows = static_cast<int64_t>(sm.entries) * blocks;
   const int64_t row0 = rows * blockIdx.x / gridDim.x, row1 = rows * (blockIdx.x + 1) / gridDim.x;
-  if (row0 >= row1) return;
+  if (row0 >= row1) {
+    pdl_wait();                                      // (the end of this kernel is the end of the one before it, too)
+    return;
+  }
   Int4Item item;
   item.left = static_cast<int>(row1 - row0);
   item.entry = static_cast<int>(row0 / blocks);
@@ -510,6 +516,7 @@ int4_matvec_kernel(const Int4Args a) {
   int4_point<kGroup, kZeros>(a, sm, blocks, units, warp, cursor);
 #pragma unroll 1
   for (int i = 0; i < kInt4Stages; ++i) int4_fetch<kGroup, kZeros>(a, sm, blocks, units, warp, lane, cursor);
+  pdl_wait();
   int before = kInt4MaxLog, entry = -1;
   uint32_t tail = 0;
   do {
@@ -531,6 +538,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 int4_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
                     T* __restrict__ out, int64_t tokens, int k, int experts, int outputs) {
+  pdl_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int64_t t = i / outputs;
   if (t >= tokens) return;
@@ -545,7 +553,7 @@ int4_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids
 }
 
 template <typename T, int kGroup, bool kZeros>
-static int int4_launch(Int4Args a, int64_t slots, cudaStream_t stream) {
+static int int4_launch(Int4Args a, int64_t slots, bool after, cudaStream_t stream) {  // after: programmatic dependent launch
   static int sms[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return STK_ERR_LAUNCH;
@@ -569,22 +577,45 @@ static int int4_launch(Int4Args a, int64_t slots, cudaStream_t stream) {
   for (int64_t first = 0; first < slots; first += kInt4MaxSlots) {
     a.first_slot = static_cast<int>(first);
     a.slots = static_cast<int>(slots - first < kInt4MaxSlots ? slots - first : kInt4MaxSlots);
-    kernel<<<static_cast<unsigned>(sms[dev]), kInt4Threads, bytes(units), stream>>>(a);
+    if (after && first == 0)
+      launch_dependent(kernel, sms[dev], kInt4Threads, static_cast<int>(bytes(units)), stream, a);
+    else
+      kernel<<<static_cast<unsigned>(sms[dev]), kInt4Threads, bytes(units), stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return STK_ERR_LAUNCH;
   }
   return STK_OK;
 }
 template <typename T>
-static int int4_by_group(const Int4Args& a, int group, int zeros, int64_t slots, cudaStream_t stream) {
+static int int4_by_group(const Int4Args& a, int group, int zeros, int64_t slots, bool after, cudaStream_t stream) {
   if (!zeros) {
-    if (group == 32) return int4_launch<T, 32, false>(a, slots, stream);
-    if (group == 64) return int4_launch<T, 64, false>(a, slots, stream);
-    return int4_launch<T, 128, false>(a, slots, stream);
+    if (group == 32) return int4_launch<T, 32, false>(a, slots, after, stream);
+    if (group == 64) return int4_launch<T, 64, false>(a, slots, after, stream);
+    return int4_launch<T, 128, false>(a, slots, after, stream);
   }
-  if (group == 32) return int4_launch<T, 32, true>(a, slots, stream);
-  if (group == 64) return int4_launch<T, 64, true>(a, slots, stream);
-  return int4_launch<T, 128, true>(a, slots, stream);
+  if (group == 32) return int4_launch<T, 32, true>(a, slots, after, stream);
+  if (group == 64) return int4_launch<T, 64, true>(a, slots, after, stream);
+  return int4_launch<T, 128, true>(a, slots, after, stream);
 }
+
+static int int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots, int x_div,
+                       int experts, int64_t outputs, int64_t inputs, int group, int zeros, int gelu, int out_f32,
+                       int dtype, bool after, cudaStream_t stream) {
+  if (slots < 0 || x_div < 1 || experts < 1 || outputs < 1 || inputs < 1) return STK_ERR_BAD_DIMS;
+  if ((group != 32 && group != 64 && group != 128) || inputs % group) return STK_ERR_BAD_DIMS;
+  if (dtype != STK_F16 && dtype != STK_BF16) return STK_ERR_BAD_DTYPE;
+  if (slots > INT32_MAX || outputs > (1 << 20) || inputs / group > kInt4MaxGroups || experts > kInt4MaxExperts)
+    return STK_ERR_TOO_LARGE;
+  if (slots == 0) return STK_OK;
+  if (!records || !x || !ids || !out) return STK_ERR_NULL_POINTER;
+  if ((reinterpret_cast<uintptr_t>(records) | reinterpret_cast<uintptr_t>(x)) % 16) return STK_ERR_BAD_LAYOUT;
+  const Int4Args a{static_cast<const unsigned char*>(records), x, ids, out, 0, 0, x_div, experts,
+                   static_cast<int>(outputs), static_cast<int>(inputs), 0, gelu, out_f32};
+  return dtype == STK_BF16 ? int4_by_group<__nv_bfloat16>(a, group, zeros, slots, after, stream)
+                           : int4_by_group<__half>(a, group, zeros, slots, after, stream);
+}
+
+// Where the hidden activations and the second products lie in the workspace of int4_mlp.
+static size_t int4_hidden_bytes(int64_t slots, int64_t ffn) { return (static_cast<size_t>(slots) * ffn * 2 + 255) / 256 * 256; }
 
 }  // namespace stk
 
@@ -596,35 +627,40 @@ extern "C" size_t stk_b200_int4_record_bytes(int group, int zeros) {
 extern "C" int stk_b200_int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots,
                                     int x_div, int experts, int64_t outputs, int64_t inputs, int group, int zeros,
                                     int gelu, int out_f32, int dtype, void* stream) {
-  if (slots < 0 || x_div < 1 || experts < 1 || outputs < 1 || inputs < 1) return STK_ERR_BAD_DIMS;
-  if ((group != 32 && group != 64 && group != 128) || inputs % group) return STK_ERR_BAD_DIMS;
-  if (dtype != STK_F16 && dtype != STK_BF16) return STK_ERR_BAD_DTYPE;
-  if (slots > INT32_MAX || outputs > (1 << 20) || inputs / group > stk::kInt4MaxGroups || experts > stk::kInt4MaxExperts)
-    return STK_ERR_TOO_LARGE;
-  if (slots == 0) return STK_OK;
-  if (!records || !x || !ids || !out) return STK_ERR_NULL_POINTER;
-  if ((reinterpret_cast<uintptr_t>(records) | reinterpret_cast<uintptr_t>(x)) % 16) return STK_ERR_BAD_LAYOUT;
-  stk::Int4Args a{static_cast<const unsigned char*>(records), x, ids, out, 0, 0, x_div, experts,
-                  static_cast<int>(outputs), static_cast<int>(inputs), 0, gelu, out_f32};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == STK_BF16 ? stk::int4_by_group<__nv_bfloat16>(a, group, zeros, slots, s)
-                           : stk::int4_by_group<__half>(a, group, zeros, slots, s);
+  return stk::int4_matvec(records, x, ids, out, slots, x_div, experts, outputs, inputs, group, zeros, gelu, out_f32, dtype,
+                          false, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" int stk_b200_int4_combine(const float* y, const int32_t* ids, const float* weights, void* out, int64_t tokens,
-                                     int top_k, int experts, int64_t outputs, int dtype, void* stream) {
-  if (tokens < 0 || top_k < 1 || experts < 1 || outputs < 1) return STK_ERR_BAD_DIMS;
-  if (dtype != STK_F16 && dtype != STK_BF16) return STK_ERR_BAD_DTYPE;
+extern "C" size_t stk_b200_int4_mlp_workspace_bytes(int64_t slots, int64_t ffn, int64_t outputs) {
+  if (slots < 1 || ffn < 1 || outputs < 1) return 0;
+  return stk::int4_hidden_bytes(slots, ffn) + static_cast<size_t>(slots) * outputs * sizeof(float);
+}
+
+extern "C" int stk_b200_int4_mlp(const void* records1, const void* records2, const void* x, const int32_t* ids,
+                                 const float* weights, void* out, int64_t tokens, int top_k, int experts, int64_t hidden,
+                                 int64_t ffn, int64_t outputs, int group1, int zeros1, int group2, int zeros2, int dtype,
+                                 void* workspace, size_t workspace_bytes, void* stream) {
+  if (tokens < 0 || top_k < 1 || outputs < 1 || ffn < 1) return STK_ERR_BAD_DIMS;
   if (tokens == 0) return STK_OK;
-  if (!y || !ids || !weights || !out) return STK_ERR_NULL_POINTER;
-  const int64_t blocks = (tokens * outputs + 255) / 256;
-  if (blocks > INT32_MAX || outputs > (1 << 24)) return STK_ERR_TOO_LARGE;
+  if (!weights || !out) return STK_ERR_NULL_POINTER;
+  if (tokens > INT32_MAX / top_k) return STK_ERR_TOO_LARGE;
+  const int64_t slots = tokens * top_k, blocks = (tokens * outputs + 255) / 256;
+  if (blocks > INT32_MAX || ffn > (1 << 20)) return STK_ERR_TOO_LARGE;
+  if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 ||
+      workspace_bytes < stk_b200_int4_mlp_workspace_bytes(slots, ffn, outputs))
+    return STK_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  float* y = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + stk::int4_hidden_bytes(slots, ffn));
+  int rc = stk::int4_matvec(records1, x, ids, workspace, slots, top_k, experts, ffn, hidden, group1, zeros1, 1, 0, dtype, false, s);
+  if (rc != STK_OK) return rc;
+  rc = stk::int4_matvec(records2, workspace, ids, y, slots, 1, experts, outputs, ffn, group2, zeros2, 0, 1, dtype, true, s);
+  if (rc != STK_OK) return rc;
+  const int grid = static_cast<int>(blocks), width = static_cast<int>(outputs);
   if (dtype == STK_BF16)
-    stk::int4_combine_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(
-        y, ids, weights, static_cast<__nv_bfloat16*>(out), tokens, top_k, experts, static_cast<int>(outputs));
+    stk::launch_dependent(stk::int4_combine_kernel<__nv_bfloat16>, grid, 256, 0, s, y, ids, weights,
+                          static_cast<__nv_bfloat16*>(out), tokens, top_k, experts, width);
   else
-    stk::int4_combine_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(
-        y, ids, weights, static_cast<__half*>(out), tokens, top_k, experts, static_cast<int>(outputs));
+    stk::launch_dependent(stk::int4_combine_kernel<__half>, grid, 256, 0, s, y, ids, weights, static_cast<__half*>(out),
+                          tokens, top_k, experts, width);
   return cudaGetLastError() == cudaSuccess ? STK_OK : STK_ERR_LAUNCH;
 }

@@ -157,12 +157,9 @@ def _check_call(what, x, w, expert_ids):
 
 
 def _matvec(x, w, ids, x_div, gelu, out):
-    with _lib.on_device(x.device):
-        rc = _lib.load().stk_b200_int4_matvec(
-            _lib.ptr(w.records), _lib.ptr(x), _lib.ptr(ids), _lib.ptr(out), ids.numel(), x_div, w.num_experts, w.outputs,
-            w.inputs, w.group, int(w.zero_points), int(gelu), int(out.dtype == torch.float32), _lib.dtype_code(w.dtype),
-            _lib.stream_ptr(x.device))
-    _lib.check(rc, "stk_b200_int4_matvec")
+    _lib.launch("stk_b200_int4_matvec", x.device, w.records.data_ptr(), x.data_ptr(), ids.data_ptr(), out.data_ptr(),
+                ids.numel(), x_div, w.num_experts, w.outputs, w.inputs, w.group, int(w.zero_points), int(gelu),
+                int(out.dtype == torch.float32), _lib.dtype_code(w.dtype))
     return out
 
 
@@ -182,7 +179,7 @@ def int4_matvec(x, w, expert_ids=None, gelu=False):
     tokens = x.shape[0]
     ids = (torch.zeros((tokens, 1), dtype=torch.int32, device=x.device) if expert_ids is None
            else expert_ids.to(torch.int32).contiguous())
-    out = torch.empty((tokens, ids.shape[1], w.outputs), dtype=x.dtype, device=x.device)
+    out = x.new_empty((tokens, ids.shape[1], w.outputs))
     _matvec(_operand(x), w, ids, ids.shape[1], gelu, out)
     return out[:, 0] if expert_ids is None else out
 
@@ -206,14 +203,12 @@ def expert_mlp_int4(x, expert_ids, weights, w1, w2):
     if torch.is_grad_enabled() and weights.requires_grad:
         raise ValueError("expert_mlp_int4 is forward only: weights require a gradient (call it under torch.no_grad())")
     tokens, top_k = expert_ids.shape
-    dev = x.device
-    ids, weights = expert_ids.to(torch.int32).contiguous(), weights.float().contiguous()
-    hidden = _matvec(_operand(x), w1, ids, top_k, True, torch.empty((tokens * top_k, w1.outputs), dtype=x.dtype, device=dev))
-    y = _matvec(hidden, w2, ids, 1, False, torch.empty((tokens * top_k, w2.outputs), dtype=torch.float32, device=dev))
-    out = torch.empty((tokens, w2.outputs), dtype=x.dtype, device=dev)
-    with _lib.on_device(dev):
-        rc = _lib.load().stk_b200_int4_combine(
-            _lib.ptr(y), _lib.ptr(ids), _lib.ptr(weights), _lib.ptr(out), tokens, top_k, w2.num_experts, w2.outputs,
-            _lib.dtype_code(x.dtype), _lib.stream_ptr(dev))
-    _lib.check(rc, "stk_b200_int4_combine")
+    ids, weights, x = expert_ids.to(torch.int32).contiguous(), weights.float().contiguous(), _operand(x)
+    out = x.new_empty((tokens, w2.outputs))
+    ws_bytes = _lib.load().stk_b200_int4_mlp_workspace_bytes(tokens * top_k, w1.outputs, w2.outputs)
+    ws = x.new_empty(ws_bytes, dtype=torch.uint8)
+    _lib.launch("stk_b200_int4_mlp", x.device, w1.records.data_ptr(), w2.records.data_ptr(), x.data_ptr(), ids.data_ptr(),
+                weights.data_ptr(), out.data_ptr(), tokens, top_k, w1.num_experts, w1.inputs, w1.outputs, w2.outputs,
+                w1.group, int(w1.zero_points), w2.group, int(w2.zero_points), _lib.dtype_code(x.dtype), ws.data_ptr(),
+                ws_bytes)
     return out

@@ -34,54 +34,50 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
-def _same_device(what, *tensors):
-    devices = {t.device for t in tensors if t is not None}
-    if len(devices) > 1:
-        raise ValueError(f"{what}: all tensors must be on one device, got " + ", ".join(sorted(map(str, devices))))
+def _once(backward):
+    """once_differentiable for a backward pass made of kernels, at no cost where no graph of it is wanted."""
+    recorded = once_differentiable(backward)
+    return lambda ctx, *grads: (recorded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
 
 # ------------------------------------------------------------------------------ gate
+def _gate(logits, mask, top_k, score, normalize, stats):
+    tokens, experts = logits.shape
+    weights = logits.new_empty((tokens, top_k), dtype=torch.float32)
+    ids = logits.new_empty((tokens, top_k), dtype=torch.int32)
+    rows = _rows(logits)
+    _lib.launch("stk_b200_top_k_gate", logits.device, rows.data_ptr(), _ld(rows), tokens, experts, top_k, score,
+                normalize, _lib.ptr(mask), weights.data_ptr(), ids.data_ptr(), _lib.ptr(stats),
+                _lib.row_dtype_code(logits.dtype))
+    return weights, ids
+
+
 class _TopKGate(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, mask, top_k, score, normalize):
-        tokens, experts = logits.shape
-        dev = logits.device
-        weights = torch.empty((tokens, top_k), dtype=torch.float32, device=dev)
-        ids = torch.empty((tokens, top_k), dtype=torch.int32, device=dev)
-        dense = score == 0 and not normalize           # the gradient reaches every logit
-        stats = torch.empty((tokens, 2), dtype=torch.float32, device=dev) if dense and ctx.needs_input_grad[0] else None
-        rows = _rows(logits)
-        with _lib.on_device(dev):
-            rc = _lib.load().stk_b200_top_k_gate(
-                _lib.ptr(rows), _ld(rows), tokens, experts, top_k, score, int(normalize), _lib.ptr(mask),
-                _lib.ptr(weights), _lib.ptr(ids), _lib.ptr(stats), _lib.row_dtype_code(logits.dtype),
-                _lib.stream_ptr(dev))
-        _lib.check(rc, "stk_b200_top_k_gate")
+        # (the gradient of the plain softmax reaches every logit; the normalized softmax weights alone give theirs)
+        dense = score == 0 and not normalize
+        stats = logits.new_empty((logits.shape[0], 2), dtype=torch.float32) if dense else None
+        weights, ids = _gate(logits, mask, top_k, score, normalize, stats)
         ctx.mark_non_differentiable(ids)
         ctx.set_materialize_grads(False)
-        # (the normalized softmax weights alone give their gradient)
         ctx.save_for_backward(logits if dense or score == 1 else None, weights, ids, stats)
-        ctx.like = (logits.shape, logits.dtype)
-        ctx.kind = (score, normalize)
+        ctx.like = (logits.shape, logits.dtype, score, normalize)
         return weights, ids
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dweights, _):
         if dweights is None:
             return None, None, None, None, None
         logits, weights, ids, stats = ctx.saved_tensors
-        (tokens, experts), dtype = ctx.like
-        dev = weights.device
+        (tokens, experts), dtype, score, normalize = ctx.like
         dweights = dweights.contiguous()
-        dlogits = torch.empty((tokens, experts), dtype=dtype, device=dev)
+        dlogits = weights.new_empty((tokens, experts), dtype=dtype)
         rows = dlogits if logits is None else _rows(logits)
-        with _lib.on_device(dev):
-            rc = _lib.load().stk_b200_top_k_gate_backward(
-                _lib.ptr(rows), _ld(rows), tokens, experts, weights.shape[1], ctx.kind[0],
-                int(ctx.kind[1]), _lib.ptr(weights), _lib.ptr(ids), _lib.ptr(stats), _lib.ptr(dweights),
-                _lib.ptr(dlogits), _lib.row_dtype_code(dtype), _lib.stream_ptr(dev))
-        _lib.check(rc, "stk_b200_top_k_gate_backward")
+        _lib.launch("stk_b200_top_k_gate_backward", weights.device, rows.data_ptr(), _ld(rows), tokens, experts,
+                    weights.shape[1], score, normalize, weights.data_ptr(), ids.data_ptr(), _lib.ptr(stats),
+                    dweights.data_ptr(), dlogits.data_ptr(), _lib.row_dtype_code(dtype))
         return dlogits, None, None, None, None
 
 
@@ -133,11 +129,15 @@ def top_k_gate(logits, top_k, score="softmax", normalize=True, token_mask=None):
         if token_mask.dtype != torch.bool or tuple(token_mask.shape) != (tokens,):
             raise ValueError(f"top_k_gate: token_mask must be bool [{tokens}], got {token_mask.dtype} "
                              f"{tuple(token_mask.shape)}")
-        _same_device("top_k_gate", logits, token_mask)
+        if token_mask.device != logits.device:
+            raise ValueError(f"top_k_gate: the logits are on {logits.device}, the token mask on {token_mask.device}")
         token_mask = token_mask.contiguous()
     if not logits.is_cuda:
         return _host_gate(logits, token_mask, top_k, _SCORES[score], normalize)
-    return _TopKGate.apply(logits, token_mask, int(top_k), _SCORES[score], bool(normalize))
+    args = (logits, token_mask, int(top_k), _SCORES[score], int(bool(normalize)))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _TopKGate.apply(*args)
+    return _gate(*args, None)
 
 
 # ------------------------------------------------------------------------------ placement
@@ -206,18 +206,12 @@ def plan_tokens(expert_ids, num_experts, block=BLOCK, rows=None):
         raise RuntimeError("plan_tokens: reading the number of rows back cannot be captured; pass rows=plan_rows(...)")
     flat = flat.to(torch.int32).contiguous()
     length = need if rows is None else rows
-    index = torch.empty(length, dtype=torch.int32, device=dev)
-    position = torch.empty(slots, dtype=torch.int32, device=dev)
-    bin_rows = torch.empty(num_experts, dtype=torch.int32, device=dev)
-    lib = _lib.load()
-    ws_bytes = lib.stk_b200_place_workspace_bytes(slots, num_experts)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    index, position, bin_rows = flat.new_empty(length), flat.new_empty(slots), flat.new_empty(num_experts)
+    ws_bytes = _lib.load().stk_b200_place_workspace_bytes(slots, num_experts)
+    ws = flat.new_empty(ws_bytes // 4) if ws_bytes else None
     word = _host_word() if rows is None else None
-    with _lib.on_device(dev):
-        rc = lib.stk_b200_place_tokens(
-            _lib.ptr(flat), slots, num_experts, block, length, int(rows is not None), _lib.ptr(index),
-            _lib.ptr(position), _lib.ptr(bin_rows), _lib.ptr(word), _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
-    _lib.check(rc, "stk_b200_place_tokens")
+    _lib.launch("stk_b200_place_tokens", dev, flat.data_ptr(), slots, num_experts, block, length, int(rows is not None),
+                index.data_ptr(), position.data_ptr(), bin_rows.data_ptr(), _lib.ptr(word), _lib.ptr(ws), ws_bytes)
     if rows is None:
         torch.cuda.current_stream(dev).synchronize()
         length = int(word)
@@ -249,30 +243,30 @@ def _host_plan(flat, num_experts, block, rows):
 # ------------------------------------------------------------------------------ rows there and back
 def _sum_rows(rows, weights, plan):
     rows = _rows(rows)
-    out = torch.empty((plan.tokens, rows.shape[1]), dtype=rows.dtype, device=rows.device)
-    with _lib.on_device(rows.device):
-        rc = _lib.load().stk_b200_sum_rows(
-            _lib.ptr(rows), _ld(rows), _lib.ptr(plan.position), _lib.ptr(weights), _lib.ptr(out), plan.tokens,
-            plan.top_k, rows.shape[1], _lib.row_dtype_code(rows.dtype), _lib.stream_ptr(rows.device))
-    _lib.check(rc, "stk_b200_sum_rows")
+    hidden = rows.shape[1]
+    out = rows.new_empty((plan.tokens, hidden))
+    _lib.launch("stk_b200_sum_rows", rows.device, rows.data_ptr(), _ld(rows), plan.position.data_ptr(),
+                _lib.ptr(weights), out.data_ptr(), plan.tokens, plan.top_k, hidden, _lib.row_dtype_code(rows.dtype))
     return out
+
+
+def _sort_rows(x, plan):
+    x = _rows(x)
+    hidden = x.shape[1]
+    rows = x.new_empty((plan.rows, hidden))
+    _lib.launch("stk_b200_sort_rows", x.device, x.data_ptr(), _ld(x), rows.data_ptr(), plan.index.data_ptr(),
+                plan.position.data_ptr(), plan.tokens, plan.top_k, plan.rows, hidden, _lib.row_dtype_code(x.dtype))
+    return rows
 
 
 class _SortTokens(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
         ctx.plan = plan
-        x = _rows(x)
-        rows = torch.empty((plan.rows, x.shape[1]), dtype=x.dtype, device=x.device)
-        with _lib.on_device(x.device):
-            rc = _lib.load().stk_b200_sort_rows(
-                _lib.ptr(x), _ld(x), _lib.ptr(rows), _lib.ptr(plan.index), _lib.ptr(plan.position), plan.tokens,
-                plan.top_k, plan.rows, x.shape[1], _lib.row_dtype_code(x.dtype), _lib.stream_ptr(x.device))
-        _lib.check(rc, "stk_b200_sort_rows")
-        return rows
+        return _sort_rows(x, plan)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, drows):
         return _sum_rows(drows, None, ctx.plan), None
 
@@ -287,23 +281,21 @@ class _UnsortTokens(torch.autograd.Function):
         return _sum_rows(rows, weights, plan)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, dout):
         rows, weights = ctx.saved_tensors
         plan, (shape, dtype) = ctx.plan, ctx.like
         dout = _rows(dout)
         drows = dweights = None
         if ctx.needs_input_grad[0]:
-            drows = torch.empty(shape, dtype=dtype, device=dout.device)
+            drows = dout.new_empty(shape, dtype=dtype)
         if rows is not None:
             rows = _rows(rows)
             dweights = torch.empty_like(weights)
-        with _lib.on_device(dout.device):
-            rc = _lib.load().stk_b200_unsort_backward(
-                _lib.ptr(dout), _ld(dout), _lib.ptr(rows), 0 if rows is None else _ld(rows), _lib.ptr(weights),
-                _lib.ptr(plan.index), _lib.ptr(plan.position), _lib.ptr(drows), _lib.ptr(dweights), plan.tokens,
-                plan.top_k, plan.rows, shape[1], _lib.row_dtype_code(dtype), _lib.stream_ptr(dout.device))
-        _lib.check(rc, "stk_b200_unsort_backward")
+        _lib.launch("stk_b200_unsort_backward", dout.device, dout.data_ptr(), _ld(dout), _lib.ptr(rows),
+                    0 if rows is None else _ld(rows), _lib.ptr(weights), plan.index.data_ptr(),
+                    plan.position.data_ptr(), _lib.ptr(drows), _lib.ptr(dweights), plan.tokens, plan.top_k, plan.rows,
+                    shape[1], _lib.row_dtype_code(dtype))
         return drows, dweights, None
 
 
@@ -311,7 +303,8 @@ def _check_rows(what, t, n, name, plan):
     if t.dim() != 2 or t.shape[0] != n:
         raise ValueError(f"{what}: expected {n} rows ({name}), got {tuple(t.shape)}")
     _lib.row_dtype_code(t.dtype)
-    _same_device(what, t, plan.position)
+    if t.device != plan.position.device:
+        raise ValueError(f"{what}: the rows are on {t.device}, the plan on {plan.position.device}")
 
 
 def sort_tokens(x, plan):
@@ -320,7 +313,7 @@ def sort_tokens(x, plan):
     32 bits."""
     _check_rows("sort_tokens", x, plan.tokens, "tokens of the plan", plan)
     if x.is_cuda:
-        return _SortTokens.apply(x, plan)
+        return _SortTokens.apply(x, plan) if torch.is_grad_enabled() and x.requires_grad else _sort_rows(x, plan)
     valid = plan.index >= 0
     out = x.new_zeros((plan.rows, x.shape[1]))
     return out.index_put((torch.nonzero(valid).view(-1),),
@@ -334,13 +327,18 @@ def unsort_tokens(rows, weights, plan):
     without an expert gets 0)."""
     _check_rows("unsort_tokens", rows, plan.rows, "rows of the plan", plan)
     if weights is not None:
-        if weights.numel() != plan.tokens * plan.top_k or weights.shape[:1] != (plan.tokens,):
+        if weights.shape != (plan.tokens, plan.top_k) and (plan.top_k != 1 or weights.shape != (plan.tokens,)):
             raise ValueError(f"unsort_tokens: weights must be [{plan.tokens}, {plan.top_k}], got {tuple(weights.shape)}")
         _lib.row_dtype_code(weights.dtype)
-        _same_device("unsort_tokens", rows, weights)
-        weights = weights.reshape(plan.tokens, plan.top_k).float().contiguous()
+        if weights.device != rows.device:
+            raise ValueError(f"unsort_tokens: the rows are on {rows.device}, the weights on {weights.device}")
+        if weights.dim() == 1:
+            weights = weights[:, None]
+        weights = weights.float().contiguous()
     if rows.is_cuda:
-        return _UnsortTokens.apply(rows, weights, plan)
+        if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
+            return _UnsortTokens.apply(rows, weights, plan)
+        return _sum_rows(rows, weights, plan)
     position = plan.position.long()
     # (a gather of at least one row, so that an empty plan needs no case of its own)
     padded = torch.cat([rows.float(), torch.zeros((1, rows.shape[1]))])

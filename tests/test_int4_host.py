@@ -109,6 +109,9 @@ def test_entry_points_check_before_any_launch():
     assert call(slots=0) == 0 and call(slots=-1) == -2 and call(div=0) == -2 and call(experts=0) == -2 and call(n=0) == -2
     assert call(k=96) == -2 and call(group=16) == -2 and call(dtype=3) == -3 and call(dtype=2) == -3
     assert call(k=513 * 64) == -9 and call(experts=70000) == -9 and call(x=None) == -1 and call(x=p + 2) == -4 and call(words=p + 8) == -4
-    assert L.stk_b200_int4_combine(p, p, p, None, 4, 2, 2, 16, 1, None) == -1
-    assert L.stk_b200_int4_combine(p, p, p, p, 4, 0, 2, 16, 1, None) == -2
-    assert L.stk_b200_int4_combine(p, p, p, p, 4, 2, 2, 16, 3, None) == -3
+    mlp = lambda tokens=4, k=2, outputs=128, group=64, weights=p, ws=p, size=1 << 20, dtype=1: L.stk_b200_int4_mlp(
+        p, p, p, p, weights, p, tokens, k, 2, 128, 256, outputs, group, 0, 64, 0, dtype, ws, size, None)
+    assert mlp(tokens=0) == 0 and mlp(tokens=-1) == -2 and mlp(k=0) == -2 and mlp(outputs=0) == -2 and mlp(group=48) == -2
+    assert mlp(weights=None) == -1 and mlp(ws=None) == -7 and mlp(ws=p + 4) == -7 and mlp(size=8191) == -7
+    assert mlp(dtype=3) == -3 and mlp(tokens=1 << 31) == -9
+    assert L.stk_b200_int4_mlp_workspace_bytes(8, 256, 128) == 8192 and L.stk_b200_int4_mlp_workspace_bytes(0, 256, 128) == 0
