@@ -283,6 +283,11 @@ __device__ __forceinline__ void int4_sums(const Int4Args& a, Int4Smem<kGroup, kZ
   }
 }
 
+// (Out of line: what it needs registers for is not the main loop's.)
+__device__ __noinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatile int* stuck) {
+  return mbar_wait(bar, parity, stuck);
+}
+
 // The warp's part of an item: records [c0, c1), from the ring's stage tail % kInt4Stages on; NT tiles of 8 slots.
 // before: the last item's log.
 template <typename T, int NT, int kGroup, bool kZeros>
@@ -310,7 +315,8 @@ __device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZ
   for (int c = c0; c < c1; ++c) {
     const uint32_t from = tail % kInt4Stages;
     const Int4Record<kGroup, kZeros>& st = sm.ring[warp][from];
-    if (!mbar_wait(smem_u32(&sm.full[warp][from]), tail / kInt4Stages & 1u, &sm.stuck)) {
+    const uint32_t bar = smem_u32(&sm.full[warp][from]), parity = tail / kInt4Stages & 1u;
+    if (!mbar_try_wait(bar, parity) && !int4_wait(bar, parity, &sm.stuck)) {
       report_status(STK_ERR_DEVICE_TIMEOUT);
       cursor.more = cursor.left = 0;                 // no further copies
     }

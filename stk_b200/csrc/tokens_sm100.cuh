@@ -14,7 +14,9 @@
 #include <stdint.h>
 
 #include "../../include/stk_b200.h"
+#include "bsmm_sm100.cuh"
 #include "gate_sm100.cuh"
+#include "sm100_ptx.cuh"
 #include "status.cuh"
 
 namespace stk {
@@ -34,6 +36,7 @@ __device__ __forceinline__ int slot_expert(const int32_t* ids, int64_t s, int64_
 __global__ void __launch_bounds__(kPlaceThreads)
 place_count_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int32_t* __restrict__ hist) {
   extern __shared__ int32_t place_count[];
+  pdl_launch_dependents();
   for (int e = threadIdx.x; e < experts; e += kPlaceThreads) place_count[e] = 0;
   __syncthreads();
   const int64_t first = static_cast<int64_t>(blockIdx.x) * kPlaceSlots;
@@ -71,15 +74,6 @@ place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int bl
   int expert[kRounds];
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) expert[i] = slot_expert(ids, first + i * 32 + lane, slots, experts);
-  if (hist != nullptr) {                                   // a warp takes every kPlaceWarps-th CTA's counts
-    for (int g = warp; g < static_cast<int>(gridDim.x); g += kPlaceWarps)
-      for (int e = lane; e < experts; e += 32) {
-        const int32_t n = hist[static_cast<int64_t>(g) * experts + e];
-        if (n == 0) continue;
-        atomicAdd(&count[e], n);
-        if (g < static_cast<int>(blockIdx.x)) atomicAdd(&before[e], n);
-      }
-  }
   uint16_t* mine = by_warp + warp * experts;
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
@@ -87,6 +81,16 @@ place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int bl
     if (expert[i] >= 0 && (same & ((1u << lane) - 1)) == 0)
       mine[expert[i]] = static_cast<uint16_t>(mine[expert[i]] + __popc(same));
     __syncwarp();
+  }
+  if (hist != nullptr) {                                   // a warp takes every kPlaceWarps-th CTA's counts
+    pdl_wait();                                            // (what comes before runs beside the counting kernel)
+    for (int g = warp; g < static_cast<int>(gridDim.x); g += kPlaceWarps)
+      for (int e = lane; e < experts; e += 32) {
+        const int32_t n = hist[static_cast<int64_t>(g) * experts + e];
+        if (n == 0) continue;
+        atomicAdd(&count[e], n);
+        if (g < static_cast<int>(blockIdx.x)) atomicAdd(&before[e], n);
+      }
   }
   __syncthreads();
   for (int e = threadIdx.x; e < experts; e += kPlaceThreads) {  // counts of the warps -> slots in the warps before
@@ -373,8 +377,11 @@ extern "C" int stk_b200_place_tokens(const int32_t* ids, int64_t slots, int expe
     if (cudaGetLastError() != cudaSuccess) return STK_ERR_LAUNCH;
   }
   const size_t smem = (3 * static_cast<size_t>(experts) + 1) * sizeof(int32_t) + kPlaceWarps * static_cast<size_t>(experts) * sizeof(uint16_t);
-  place_kernel<<<static_cast<unsigned>(ctas), kPlaceThreads, smem, s>>>(ids, slots, experts, block, rows, fixed, hist,
-                                                                         index, position, bin_rows, total);
+  if (ctas > 1)
+    launch_dependent(place_kernel, static_cast<int>(ctas), kPlaceThreads, static_cast<int>(smem), s, ids, slots, experts,
+                     block, rows, fixed, hist, index, position, bin_rows, total);
+  else
+    place_kernel<<<1, kPlaceThreads, smem, s>>>(ids, slots, experts, block, rows, fixed, hist, index, position, bin_rows, total);
   return cudaGetLastError() == cudaSuccess ? STK_OK : STK_ERR_LAUNCH;
 }
 
