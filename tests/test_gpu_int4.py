@@ -224,6 +224,36 @@ def test_decoding_step_with_the_gate_and_captured():
         assert torch.equal(outputs[0], eager[a][0]) and torch.equal(outputs[1], eager[b][0])
 
 
+def test_calls_in_a_row_between_other_kernels():
+    """Launches that begin while the one before them runs out: many short calls back to back, between products and gates of
+    the same stream, give what each gives alone."""
+    import stk_b200 as stk
+    from stk_b200 import dmoe
+    experts, hidden, ffn = 4, 128, 256
+    g = torch.Generator().manual_seed(8)
+    make = lambda *shape: (torch.randn(*shape, generator=g) * 0.1).half().cuda()
+    w1, w2 = dmoe.quantize_int4(make(experts, hidden, ffn)), dmoe.quantize_int4(make(experts, ffn, hidden))
+    topo = dmoe.topology_from_bins(torch.ones(experts, dtype=torch.int32, device="cuda"), experts, ffn, torch.float16, "cuda")
+    a, b = make(experts * 128, hidden), make(hidden, experts * ffn)
+    batches = [(make(t, hidden) * 10, torch.randint(-1, experts, (t, 2), generator=g).cuda(), torch.rand(t, 2, generator=g).cuda())
+               for t in (1, 3, 150, 17)]
+
+    def step(x, ids, weights):
+        out = dmoe.expert_mlp_int4(x, ids, weights, w1, w2)
+        product = stk.ops.sdd(a, b, topo).data
+        plan = dmoe.plan_tokens(ids.repeat(30, 1), experts, rows=dmoe.plan_rows(60 * len(ids), experts))
+        return out, dmoe.int4_matvec(x, w1, ids), product, plan.position
+
+    alone = []
+    for batch in batches:
+        torch.cuda.synchronize()
+        alone.append(step(*batch))
+        torch.cuda.synchronize()
+    for _ in range(50):
+        for batch, expect in zip(batches, alone):
+            assert all(torch.equal(p, q) for p, q in zip(step(*batch), expect))
+
+
 def test_quantized_experts_stay_near_the_16_bit_ones():
     """quantize_int4 takes dmoe.expert_mlp's weights in the documented views: the two forms of the layer agree up to what
     4 bits lose.  Every weight is off by half a scale at most, a scale being a seventh of the group's largest

@@ -306,6 +306,40 @@ def test_rows_take_views_and_weights_of_other_kinds():
     assert torch.equal(dmoe.unsort_tokens(dmoe.sort_tokens(x, flat), torch.ones(90, device="cuda"), flat), x)
 
 
+def test_rows_of_plans_without_slots():
+    """No slot has an expert: no row at all, or only padding."""
+    from stk_b200 import dmoe
+    none = torch.full((5, 2), -1, device="cuda")
+    for ids, rows in ((none, None), (none, 1024), (none[:0], None), (none[:0], 256)):
+        plan = dmoe.plan_tokens(ids, 4, rows=rows)
+        assert plan.rows == (rows or 0) and bool((plan.index == -1).all()) and bool((plan.position == -1).all())
+        assert plan.bin_rows.tolist() == [0, 0, 0, plan.block_rows]
+        x = torch.randn(len(ids), 40, device="cuda", requires_grad=True)
+        w = torch.rand(len(ids), 2, device="cuda", requires_grad=True)
+        moved = dmoe.sort_tokens(x, plan)
+        assert moved.shape == (plan.rows, 40) and not bool(moved.any())
+        leaf = torch.full((plan.rows, 40), torch.nan, device="cuda", requires_grad=True)
+        out = dmoe.unsort_tokens(leaf, w, plan)
+        assert out.shape == x.shape and not bool(out.any())
+        grads = torch.autograd.grad(out, (leaf, w), torch.ones_like(out))
+        assert not bool(grads[0].any()) and not bool(grads[1].any())
+        assert not bool(torch.autograd.grad(moved, x, torch.ones_like(moved))[0].any())
+
+
+def test_backward_accumulates_and_takes_shared_use():
+    """The same rows and weights used twice, and .backward() into leaves that hold gradients already."""
+    from stk_b200 import dmoe
+    plan, g = rows_case(50, 24, 3, 2, torch.float32)
+    x = torch.randn(50, 24, generator=g).cuda().requires_grad_()
+    w = torch.rand(50, 2, generator=g).cuda().requires_grad_()
+    moved = dmoe.sort_tokens(x, plan)
+    once = torch.autograd.grad(dmoe.unsort_tokens(moved, w, plan).sum(), (x, w), retain_graph=True)
+    for _ in range(2):
+        (dmoe.unsort_tokens(moved, w, plan).sum() + dmoe.unsort_tokens(moved, w, plan).sum()).backward(retain_graph=True)
+    torch.testing.assert_close(x.grad, 4 * once[0], rtol=1e-6, atol=1e-6)
+    torch.testing.assert_close(w.grad, 4 * once[1], rtol=1e-6, atol=1e-6)
+
+
 def test_rows_beyond_32_bit_offsets():
     from stk_b200 import dmoe
     tokens, hidden, top_k = 290000, 4096, 2               # 580000 rows and padding: 2.4e9 elements
