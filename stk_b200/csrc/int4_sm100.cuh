@@ -25,6 +25,11 @@
 // to a record's rows; 16 / that many warps cut each row along the inputs, and their sums are joined in shared memory, in
 // order.  Each warp streams its records through a ring of its own, by bulk copies that one lane starts; the copies run
 // ahead across the items.
+//
+// 32 slots on 8 experts of 4096 inputs x 14336 outputs, bf16, group 128 (242 MB, 37 us of HBM time): 58 - 62 us, of which the
+// copies alone take 41 and the arithmetic alone 49.  The arithmetic is 16.5 instructions for a word of 8 codes a lane,
+// 9.4 of them on the integer pipe.  Measured and no better: two rows of records per warp sharing their loads of x, 24
+// warps of 80 registers, a ring of 4, shifts by multiplication.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -43,8 +48,8 @@ namespace stk {
 constexpr int kInt4Warps = 16;
 constexpr int kInt4Threads = 32 * kInt4Warps;
 constexpr int kInt4Strips = 2;                      // strips of a record
-constexpr int kInt4Rows = 16 * kInt4Strips;
-constexpr int kInt4Inputs = 128;
+constexpr int kInt4Rows = 16 * kInt4Strips;         // output rows of a record
+constexpr int kInt4Inputs = 128;                    // inputs of a record
 constexpr int kInt4Stages = 2;                      // records of a warp's ring
 constexpr int kInt4MaxExperts = 1024;
 constexpr int kInt4MaxSlots = 256;                  // of one launch

