@@ -1,8 +1,9 @@
 """The gate, the token placement and the rows' ways on the GPU, against plain 64-bit statements (tests/routing_reference.py).
 
 Tolerances, with u = 2^-24 (one rounding to 32 bits) and h = half a step of the output's type:
-* gate weights: relative 128 u.  The exponent's argument l - max is rounded once, an error of |l - max| u of the exponential (|l - max| < 40
-  for the logits here); the exponential itself adds 2 roundings, the sum over a row at most 32 + 5, the division 2.
+* gate weights: relative 128 u.  The exponent's argument l - max and its product with log2(e) are rounded once each, errors
+  of |l - max| u of the exponential (|l - max| < 40 for the logits here); the power of two is 4 u off, the sum over a
+  row adds at most 32 + 5, the division 2.
 * gate gradient: h |d| for its type, and 256 u w_i (|g_i| + sum |g_j| w_j): the same errors in every term of a difference.
 * sums over choices: h |out| and (k + 1) u times the sum of the terms' magnitudes.
 * dot products: (h / 32 + 16) u times the sum of the magnitudes: a lane adds at most hidden / 32 terms, then come
