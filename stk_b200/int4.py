@@ -9,6 +9,7 @@ The reference has no counterpart.
 import torch
 
 from stk_b200.backend import lib as _lib
+from stk_b200.routing import ids32
 
 GROUPS = (32, 64, 128)
 MAX_EXPERTS = 1024
@@ -179,7 +180,7 @@ def int4_matvec(x, w, expert_ids=None, gelu=False):
         raise ValueError(f"int4_matvec: {w.num_experts} experts need expert_ids")
     tokens = x.shape[0]
     ids = (torch.zeros((tokens, 1), dtype=torch.int32, device=x.device) if expert_ids is None
-           else expert_ids.to(torch.int32).contiguous())
+           else ids32(expert_ids))
     out = x.new_empty((tokens, ids.shape[1], w.outputs))
     _matvec(_operand(x), w, ids, ids.shape[1], gelu, out)
     return out[:, 0] if expert_ids is None else out
@@ -204,7 +205,7 @@ def expert_mlp_int4(x, expert_ids, weights, w1, w2):
     if torch.is_grad_enabled() and weights.requires_grad:
         raise ValueError("expert_mlp_int4 is forward only: weights require a gradient (call it under torch.no_grad())")
     tokens, top_k = expert_ids.shape
-    ids, weights, x = expert_ids.to(torch.int32).contiguous(), weights.float().contiguous(), _operand(x)
+    ids, weights, x = ids32(expert_ids), weights.float().contiguous(), _operand(x)
     out = x.new_empty((tokens, w2.outputs))
     ws_bytes = _lib.load().stk_b200_int4_mlp_workspace_bytes(tokens * top_k, w1.outputs, w2.outputs)
     ws = x.new_empty(ws_bytes, dtype=torch.uint8)

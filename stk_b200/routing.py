@@ -34,6 +34,13 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
+def ids32(ids):
+    """Expert ids as contiguous int32; 64-bit ones beyond it stay beyond every expert."""
+    if ids.dtype == torch.int64:
+        ids = ids.clamp(-1, 2 ** 31 - 1)
+    return ids.to(torch.int32).contiguous()
+
+
 def _once(backward):
     """once_differentiable for a backward pass made of kernels, at no cost where no graph of it is wanted."""
     recorded = once_differentiable(backward)
@@ -188,6 +195,7 @@ def plan_tokens(expert_ids, num_experts, block=BLOCK, rows=None):
         raise ValueError(f"plan_tokens: 1 to {MAX_EXPERTS} experts, got {num_experts}")
     if block < 1:
         raise ValueError(f"plan_tokens: block must be positive, got {block}")
+    num_experts, block, rows = int(num_experts), int(block), None if rows is None else int(rows)
     tokens = expert_ids.shape[0]
     top_k = 1 if expert_ids.dim() == 1 else expert_ids.shape[1]
     if top_k < 1:
@@ -204,7 +212,7 @@ def plan_tokens(expert_ids, num_experts, block=BLOCK, rows=None):
     dev = flat.device
     if rows is None and torch.cuda.is_current_stream_capturing():
         raise RuntimeError("plan_tokens: reading the number of rows back cannot be captured; pass rows=plan_rows(...)")
-    flat = flat.to(torch.int32).contiguous()
+    flat = ids32(flat)
     length = need if rows is None else rows
     index, position, bin_rows = flat.new_empty(length), flat.new_empty(slots), flat.new_empty(num_experts)
     ws_bytes = _lib.load().stk_b200_place_workspace_bytes(slots, num_experts)

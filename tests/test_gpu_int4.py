@@ -140,8 +140,9 @@ def test_experts_that_do_not_exist_are_reported():
     y = dmoe.int4_matvec(x, w, torch.tensor([[0], [3], [1], [-1]], device="cuda"))
     assert lib.device_status() == -2 and lib.device_status() == 0
     assert not bool(y[1].any()) and not bool(y[3].any()) and bool(y[0].any())
-    y = dmoe.int4_matvec(x[:1], w, torch.tensor([[77]], device="cuda"))
-    assert lib.device_status() == -2 and not bool(y.any())
+    for far in (77, 2 ** 32, 2 ** 33 + 1):
+        y = dmoe.int4_matvec(x[:1], w, torch.tensor([[far]], device="cuda"))
+        assert lib.device_status() == -2 and not bool(y.any())
 
 
 def mlp64(x, ids, weights, first, second):

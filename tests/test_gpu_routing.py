@@ -156,6 +156,8 @@ def test_plan_reports_experts_that_do_not_exist():
     plan = dmoe.plan_tokens(torch.tensor([0, 5, 1, 99, 4], device="cuda"), 5)
     assert lib.device_status() == -2 and lib.device_status() == 0
     assert plan.position.tolist() == [0, -1, 128, -1, 256]       # as if they had none
+    plan = dmoe.plan_tokens(torch.tensor([2 ** 32, 1, 2 ** 33 + 2, -2 ** 33], device="cuda"), 5)  # 0, 1, 2, 0 in 32 bits
+    assert lib.device_status() == -2 and plan.position.tolist() == [-1, 0, -1, -1]
 
 
 def test_plans_of_two_threads_at_once():
