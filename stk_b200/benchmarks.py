@@ -3,7 +3,8 @@
     python -m stk_b200.benchmarks c2     # dMoE forward + backward products, 16 experts with Zipf token counts, bf16
     python -m stk_b200.benchmarks c3     # random block sparsity on 8192^3, bf16, all op / transpose combinations
     python -m stk_b200.benchmarks meta   # metadata / conversion / row-movement kernels: achieved GB/s
-    python -m stk_b200.benchmarks train  # forward + backward of the experts' MLP, fused against unfused
+    python -m stk_b200.benchmarks train  # forward + backward of the experts' MLP, fused against unfused, and of the whole layer
+    python -m stk_b200.benchmarks decode # the experts' MLP on few tokens: 4-bit weights against 16-bit ones in padded bins
     python -m stk_b200.benchmarks ref    # the reference's own Triton kernels on this GPU (needs oracle/_ref)
     python -m stk_b200.benchmarks single 0.25   # a few launches on one random topology (profiler case)
 
@@ -311,6 +312,61 @@ def train_step(dev="cuda"):
         print(f"{name:32s} fwd+bwd {ms * 1e3:7.1f} us  {flops / ms / 1e9:5.0f} TFLOP/s")
 
 
+def layer_step(dev="cuda"):
+    """Forward + backward of a whole dMoE layer on the same shape with top-2 routing: gate, placement, sorted tokens,
+    experts' MLP and weighted return, every gradient.  With as many rows as the batch needs (read back) and with the
+    number of rows fixed in advance, the latter also replayed from a CUDA graph."""
+    T, h, f, E, k, dtype = 16384, 1024, 4096, 8, 2, torch.float16
+    rand = lambda *shape: torch.empty(*shape, dtype=dtype, device=dev).normal_(0, 0.02).requires_grad_(True)
+    leaves = (rand(T, h), rand(h, E), rand(h, E * f), rand(E * f, h))
+    dout = torch.empty(T, h, dtype=dtype, device=dev).normal_(0, 0.02)
+    most = dmoe.plan_rows(T * k, E)
+
+    def step(rows=None):
+        x, router, w1, w2 = leaves
+        weights, ids = dmoe.top_k_gate(x @ router, k)
+        plan = dmoe.plan_tokens(ids, E, rows=rows)
+        topo = dmoe.topology_from_bins(plan.bin_rows, plan.block_rows, f, dtype, x.device, materialize=False)
+        out = dmoe.unsort_tokens(dmoe.expert_mlp(dmoe.sort_tokens(x, plan), w1, w2, topo), weights, plan)
+        return plan, torch.autograd.grad(out, leaves, dout)
+
+    step(most), step(most)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(most)
+    rows = step()[0].rows
+    for name, n, fn in (("layer, rows read back", rows, step), ("layer, fixed rows", most, lambda: step(most)),
+                        ("layer, fixed rows, graph", most, graph.replay)):
+        ms = _time_ms(fn, iters=10, warm=3)
+        flops = 6 * 2.0 * n * f * h
+        print(f"{name:32s} fwd+bwd {ms * 1e3:7.1f} us  {flops / ms / 1e9:5.0f} TFLOP/s of the six products ({n} rows)")
+
+
+def decode(dev="cuda", experts=8, hidden=4096, ffn=14336, top_k=2, group=128):
+    """The experts' MLP of one dMoE layer on few tokens (bf16, weights of 1.9 GB in 16 bits): dmoe.expert_mlp_int4 against
+    the 16-bit products on padded bins, each with all that its step takes from the choices on."""
+    rand = lambda *shape: torch.empty(*shape, dtype=torch.bfloat16, device=dev).normal_(0, 0.02)
+    w1, w2 = rand(hidden, experts * ffn), rand(experts * ffn, hidden)
+    q1 = dmoe.quantize_int4(w1.view(hidden, experts, ffn).transpose(0, 1), group)
+    q2 = dmoe.quantize_int4(w2.view(experts, ffn, hidden), group)
+    print("| tokens | experts in use | 4-bit us | GB/s of 4-bit weights | 16-bit us |\n|---|---|---|---|---|")
+    for tokens in (1, 4, 16, 64, 128):
+        x = rand(tokens, hidden)
+        weights, ids = dmoe.top_k_gate(torch.randn(tokens, experts, device=dev), top_k)
+        used = int(ids.unique().numel())
+
+        def wide():
+            plan = dmoe.plan_tokens(ids, experts, rows=dmoe.plan_rows(tokens * top_k, experts))
+            topo = dmoe.topology_from_bins(plan.bin_rows, plan.block_rows, ffn, x.dtype, x.device, materialize=False)
+            y = stk.ops.dsd(stk.ops.sdd_gelu(dmoe.sort_tokens(x, plan), w1, topo), w2)
+            return dmoe.unsort_tokens(y, weights, plan)
+
+        ms = time_interleaved({"int4": lambda: dmoe.expert_mlp_int4(x, ids, weights, q1, q2), "wide": wide}, iters=10)
+        bytes_read = 2.0 * used * hidden * ffn * (0.5 + 2.0 / group)
+        print(f"| {tokens} | {used} | {ms['int4'] * 1e3:.1f} | {bytes_read / ms['int4'] / 1e6:.0f} | {ms['wide'] * 1e3:.1f} |",
+              flush=True)
+
+
 def products_fp8(dev="cuda", experts=8, rows_per_expert=4096, hidden=4096, ffn=14336):
     """The forward products of one GPU's share of the dMoE-XL layer (BASELINE configs[4] / 8) with
     float8_e4m3fn operands against the same products in bfloat16 and against cuBLASLt's float8 GEMM
@@ -389,12 +445,15 @@ if __name__ == "__main__":
     which = sys.argv[1] if len(sys.argv) > 1 else "c2"
     if which == "train":
         train_step()
+        layer_step()
     elif which == "ref":
         reference_triton()
     else:
         with torch.no_grad():
             if which == "single":
                 single(float(sys.argv[2]) if len(sys.argv) > 2 else 0.25)
+            elif which == "decode":
+                decode()
             elif which == "meta":
                 for r in meta_kernels(peak_gbs=6549.4):
                     print(f"| {r['kernel']} | {r['algorithmic_mb']} | {r['us']} | {r['gbs']} | {r['frac']} | {r['note']} |", flush=True)
