@@ -8,6 +8,10 @@ with its gradient.  Public as stk_b200.dmoe.top_k_gate / plan_rows / plan_tokens
     y = dmoe.expert_mlp(dmoe.sort_tokens(x, plan), w1, w2, topo)
     out = dmoe.unsort_tokens(y, weights, plan)             # differentiable in x, w_router, w1 and w2
 
+A step with its backward pass can be captured in a CUDA graph (plan_tokens with rows=...) as long as no eager graph of the
+same leaves is alive that was made on the default stream: torch's engine waits for the stream of a leaf's accumulator,
+in torch.autograd.grad too, and raises an error where that is not the capturing one.
+
 On CUDA tensors everything runs as kernels of libstk_b200.so.  Host tensors take plain torch operations (as in
 stk_b200.dmoe: for tests, not for production use).  The reference is a matmul library and has no counterpart.
 """
