@@ -718,8 +718,8 @@ static int device_info(DeviceInfo** out) {
 }
 
 // Launch with programmatic stream serialization: the kernel's set-up (barriers, TMEM allocation) may
-// overlap the tail of the kernel before it in the stream; it waits (griddepcontrol.wait) before its
-// first global read.
+// overlap the tail of the kernel before it in the stream; it waits (griddepcontrol.wait) before it
+// touches what that kernel reads or writes.
 template <typename... Params, typename... Args>
 static cudaError_t launch_dependent(void (*kernel)(Params...), int grid, int block, int smem_bytes,
                                     cudaStream_t stream, const Args&... args) {

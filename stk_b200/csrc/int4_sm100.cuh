@@ -254,7 +254,7 @@ struct Int4Inputs {
   __device__ __forceinline__ void load(const Int4Args& a, int c, int quarter, uint4 (&to)[NT]) const {
     const int at = kGroup == 128 || c * kInt4Inputs + quarter * 32 < a.inputs ? 4 * quarter : 0;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) to[n] = __ldg(reinterpret_cast<const uint4*>(x[n]) + at);
+    for (int n = 0; n < NT; ++n) to[n] = load_written(reinterpret_cast<const uint4*>(x[n]) + at);
   }
 };
 
@@ -547,7 +547,7 @@ int4_matvec_kernel(const Int4Args a) {
 // out[t] = sum_j weights[t, j] * y[t * k + j] over the choices that have an expert; y in 32 bits.
 template <typename T>
 __global__ void __launch_bounds__(256)
-int4_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
+int4_combine_kernel(const float* y, const int32_t* __restrict__ ids, const float* __restrict__ weights,
                     T* __restrict__ out, int64_t tokens, int k, int experts, int outputs) {
   pdl_wait();
   const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
@@ -558,7 +558,7 @@ int4_combine_kernel(const float* __restrict__ y, const int32_t* __restrict__ ids
   for (int j = 0; j < k; ++j) {
     const int64_t s = t * k + j;
     const int e = ids[s];
-    if (e >= 0 && e < experts) acc = fmaf(weights[s], y[s * outputs + n], acc);
+    if (e >= 0 && e < experts) acc = fmaf(weights[s], load_written(y + s * outputs + n), acc);
   }
   out[i] = from_f32<T>(acc);
 }

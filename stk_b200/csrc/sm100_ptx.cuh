@@ -99,12 +99,32 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 // ---------------------------------------------------------------- programmatic dependent launch
 // A kernel launched with the programmatic-stream-serialization attribute may start while the kernel
-// before it in the stream still runs; it must not touch global memory before pdl_wait(), which
-// returns once that kernel has completed and its writes are visible.  pdl_launch_dependents() lets
-// the NEXT kernel's CTAs be scheduled as soon as SMs free up.  Both are no-ops in an ordinary launch.
+// before it in the stream still runs.  pdl_wait() returns once that kernel has completed and its writes
+// are visible; before it, a kernel reads nothing that the kernel before it writes, and writes nothing
+// that it reads or writes.  pdl_launch_dependents() lets the NEXT kernel's CTAs be scheduled as soon as
+// SMs free up.  Both are no-ops in an ordinary launch.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Loads, behind pdl_wait(), of what the kernel before wrote while this one was already running.  That data is not
+// read-only for this kernel's lifetime, so the read-only path (__ldg, or a const __restrict__ pointer) is not for it: a
+// compiler may move such a load over the wait.  These stay behind it: volatile statements keep their order.
+__device__ __forceinline__ uint4 load_written(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ float load_written(const float* p) {
+  float v;
+  asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ int32_t load_written(const int32_t* p) {
+  int32_t v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
 }
 
 // ---------------------------------------------------------------- TMA

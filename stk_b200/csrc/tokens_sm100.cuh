@@ -58,7 +58,7 @@ place_count_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, 
 // within the bins included), written to memory that the host reads.
 __global__ void __launch_bounds__(kPlaceThreads)
 place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int block, int64_t rows, int fixed,
-             const int32_t* __restrict__ hist, int32_t* __restrict__ index, int32_t* __restrict__ position,
+             const int32_t* hist, int32_t* __restrict__ index, int32_t* __restrict__ position,
              int32_t* __restrict__ bin_rows, int64_t* __restrict__ total) {
   extern __shared__ int32_t place_smem[];
   int32_t* count = place_smem;                             // [experts] slots of all CTAs
@@ -87,7 +87,7 @@ place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int bl
     pdl_wait();                                            // (what comes before runs beside the counting kernel)
     for (int g = warp; g < static_cast<int>(gridDim.x); g += kPlaceWarps)
       for (int e = lane; e < experts; e += 32) {
-        const int32_t n = hist[static_cast<int64_t>(g) * experts + e];
+        const int32_t n = load_written(hist + static_cast<int64_t>(g) * experts + e);
         if (n == 0) continue;
         atomicAdd(&count[e], n);
         if (g < static_cast<int>(blockIdx.x)) atomicAdd(&before[e], n);
