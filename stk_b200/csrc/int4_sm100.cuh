@@ -5,11 +5,14 @@
 // The bytes of the chosen experts' weights are the floor: a weight is half a byte, so at 6.5 TB/s an SM has to take in 46
 // weights a clock, more than it could convert and multiply on the CUDA cores in 32 bits (three instructions a weight).
 // So the products run as mma.m16n8k16: 16 output rows x 16 inputs of weights against 8 slots, sums in 32 bits.  The A
-// operand is 16 + code, a 16-bit float made by putting an exponent above the code's four bits (exact, one shift and one
-// logical instruction for two weights).  sum (code - zero) x = sum (16 + code) x - (16 + zero) sum x: the sums of the
-// inputs, a table in shared memory made once for each (expert, tile of slots) by products with ones, are where the sum of
-// a group starts from, and the scale multiplies what comes out.  All of it is in 32 bits; nothing is rounded before the
-// result.  (An infinity among the inputs therefore makes a NaN.)
+// operand is code - zero: putting an exponent above the code's four bits makes 16 + code, a 16-bit float (one shift and one
+// logical instruction for two weights), and a packed subtraction takes 16 + zero away (one more); both are exact.  The
+// scale multiplies a group's sum.  So the only roundings are those of sums of (code - zero) x and of scaled group sums, in 32
+// bits, and that of the result: the error goes by sum |w x|, and an input whose code is the zero point adds exactly nothing.
+// (Summing (16 + code) x and taking (16 + zero) sum x away from the sum instead is cheaper by the subtractions and dearer by
+// a table of input sums, and its error goes by sum (32 + code + zero) |scale x|, which outliers among the inputs make
+// large.)  An infinity among the inputs makes its results infinite or NaN; so do finite ones whose sum of (code - zero) x
+// over a group is beyond the range of 32 bits (bf16 inputs above 1e35).
 //
 // Layout (made once, by the host): a record holds 32 output rows (two strips of 16) x 128 inputs, in the order in which
 // the kernel reads them.  First the codes, strip by strip, 64 inputs at a time, 512 bytes in the order in which the lanes
@@ -133,14 +136,17 @@ struct Int4Smem {
   int32_t entries;
   int32_t dropped;
   int32_t stuck;
-  alignas(16) float sums[1];                        // [groups][8 * kInt4MaxTiles]: of the entry's slots' inputs
 };
 
 template <typename T> struct Int4Type;
 template <> struct Int4Type<__nv_bfloat16> {
   static constexpr uint32_t kMagic = 0x41804180u;  // 16, with steps of 1 from bit 3 on
   static constexpr int kBit = 3;
-  static constexpr uint32_t kOnes = 0x3f803f80u;
+  static constexpr uint32_t kOffset = 0x41c041c0u;  // 24: the magic number and a zero point of 8
+  __device__ static uint32_t minus(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
   __device__ static float2 pair(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v)); }
   __device__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -156,7 +162,11 @@ template <> struct Int4Type<__nv_bfloat16> {
 template <> struct Int4Type<__half> {
   static constexpr uint32_t kMagic = 0x4c004c00u;  // 16, with steps of 1 from bit 6 on
   static constexpr int kBit = 6;
-  static constexpr uint32_t kOnes = 0x3c003c00u;
+  static constexpr uint32_t kOffset = 0x4e004e00u;  // 24
+  __device__ static uint32_t minus(uint32_t a, uint32_t b) {
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&d);
+  }
   __device__ static float2 pair(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
   __device__ static void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -170,14 +180,18 @@ template <> struct Int4Type<__half> {
   }
 };
 
-// 16 + code for the 8 codes of a word, as the A operand of one product.  mask and magic are registers (int4_constant):
-// one logical instruction takes one immediate, and with two constants known to it the compiler makes two of it (14
-// instead of 7 integer instructions a word).
+// code - zero for the 8 codes of a word, as the A operand of one product; lo and hi are 16 + zero of rows g and g + 8.  mask
+// and magic are registers (int4_constant): one logical instruction takes one immediate, and with two constants known to it
+// the compiler makes two of it (14 instead of 7 integer instructions a word).
 template <typename T>
-__device__ __forceinline__ void int4_decode(uint32_t w, uint32_t mask, uint32_t magic, uint32_t (&a)[4]) {
+__device__ __forceinline__ void int4_decode(uint32_t w, uint32_t mask, uint32_t magic, uint32_t lo, uint32_t hi,
+                                            uint32_t (&a)[4]) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(a[i]) : "r"(__funnelshift_r(w, w, 4 * i)), "r"(mask), "r"(magic));
+  for (int i = 0; i < 4; ++i) {
+    uint32_t v;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(v) : "r"(__funnelshift_r(w, w, 4 * i)), "r"(mask), "r"(magic));
+    a[i] = Int4Type<T>::minus(v, i % 2 ? hi : lo);
+  }
 }
 __device__ __forceinline__ uint32_t int4_constant(uint32_t v) {
   uint32_t r;
@@ -258,36 +272,6 @@ struct Int4Inputs {
   }
 };
 
-// The table of an entry's sums of inputs, a group each; without zero points, -(16 + 8) times them.
-template <typename T, int NT, int kGroup, bool kZeros>
-__device__ __forceinline__ void int4_sums(const Int4Args& a, Int4Smem<kGroup, kZeros>& sm, int entry, int units, int warp,
-                                          int lane) {
-  const uint32_t ones[4] = {Int4Type<T>::kOnes, Int4Type<T>::kOnes, Int4Type<T>::kOnes, Int4Type<T>::kOnes};
-  constexpr int kPer = kGroup / 32;
-  for (int c = warp; c < units; c += kInt4Warps) {
-    const Int4Inputs<T, NT, kGroup, kZeros> in(a, sm, sm.entry_first[entry], sm.entry_slots[entry], c, lane);
-    uint4 v[4][NT];
-#pragma unroll
-    for (int h = 0; h < 4; ++h) in.load(a, c, h, v[h]);
-    float sum[NT][4];
-#pragma unroll
-    for (int h = 0; h < 4; ++h) {
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (h % kPer == 0) sum[n][0] = sum[n][1] = sum[n][2] = sum[n][3] = 0.0f;
-        Int4Type<T>::mma(sum[n], ones, v[h][n].x, v[h][n].y);
-        Int4Type<T>::mma(sum[n], ones, v[h][n].z, v[h][n].w);
-        const int group = c * (kInt4Inputs / kGroup) + h / kPer;
-        if (h % kPer == kPer - 1 && lane < 4) {       // (every row of the product is the sum)
-          float* to = &sm.sums[(group * kInt4MaxTiles + n) * 8 + 2 * lane];
-          to[0] = kZeros ? sum[n][0] : -24.0f * sum[n][0];
-          to[1] = kZeros ? sum[n][1] : -24.0f * sum[n][1];
-        }
-      }
-    }
-  }
-}
-
 // (Out of line: what it needs registers for is not the main loop's.)
 __device__ __noinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatile int* stuck) {
   return mbar_wait(bar, parity, stuck);
@@ -309,6 +293,9 @@ __device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZ
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[r][n][i] = 0.0f;
   const uint32_t mask = int4_constant(0x000f000fu << Int4Type<T>::kBit), magic = int4_constant(Int4Type<T>::kMagic);
+  uint32_t lo[kInt4Strips], hi[kInt4Strips];         // 16 + zero, twice
+#pragma unroll
+  for (int r = 0; r < kInt4Strips; ++r) lo[r] = hi[r] = Int4Type<T>::kOffset;
   // x runs kAhead quarters (of 32 inputs) ahead, across the records
   constexpr int kAhead = NT == 1 ? 4 : 2;
   uint4 xq[kAhead][NT];
@@ -316,7 +303,6 @@ __device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZ
 #pragma unroll
     for (int h = 0; h < kAhead; ++h) in.load(a, c0, h, xq[h]);
   }
-  const float* sums = sm.sums + c0 * (kInt4Inputs / kGroup) * kInt4MaxTiles * 8 + 2 * t;
   for (int c = c0; c < c1; ++c) {
     const uint32_t from = tail % kInt4Stages;
     const Int4Record<kGroup, kZeros>& st = sm.ring[warp][from];
@@ -333,35 +319,29 @@ __device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZ
 #pragma unroll
         for (int r = 0; r < kInt4Strips; ++r) q[r] = st.words[r][h / 2][lane];
       }
-      float2 sum[NT];
-      if (h % kPer == 0) {                           // a new group
+      if constexpr (kZeros) {
+        if (h % kPer == 0) {                         // a new group
+          constexpr uint32_t kTwice = 0x00010001u << Int4Type<T>::kBit;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) sum[n] = *reinterpret_cast<const float2*>(sums + (h / kPer * kInt4MaxTiles + n) * 8);
+          for (int r = 0; r < kInt4Strips; ++r) {
+            const uint32_t z = st.zeros[h / kPer][r][g];
+            lo[r] = (z & 0xffu) * kTwice + magic;
+            hi[r] = (z >> 8) * kTwice + magic;
+          }
+        }
       }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int r = 0; r < kInt4Strips; ++r) {
           uint32_t w[4];
-          int4_decode<T>(h % 2 ? (u ? q[r].w : q[r].z) : (u ? q[r].y : q[r].x), mask, magic, w);
-          float zero_lo = 1.0f, zero_hi = 1.0f;
-          if constexpr (kZeros) {
-            if (h % kPer == 0 && u == 0) {
-              const uint32_t z = st.zeros[h / kPer][r][g];
-              zero_lo = -16.0f - static_cast<float>(z & 0xffu);
-              zero_hi = -16.0f - static_cast<float>(z >> 8);
-            }
-          }
+          int4_decode<T>(h % 2 ? (u ? q[r].w : q[r].z) : (u ? q[r].y : q[r].x), mask, magic, lo[r], hi[r], w);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             const uint4& v = xq[h % kAhead][n];
             if (h % kPer == 0 && u == 0) {
-              float start[4] = {sum[n].x, sum[n].y, sum[n].x, sum[n].y};
-              if (kZeros) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) start[i] *= i < 2 ? zero_lo : zero_hi;
-              }
-              Int4Type<T>::mma_from(part[r][n], w, v.x, v.y, start);
+              const float zero[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              Int4Type<T>::mma_from(part[r][n], w, v.x, v.y, zero);
             } else {
               Int4Type<T>::mma(part[r][n], w, u ? v.z : v.x, u ? v.w : v.y);
             }
@@ -382,7 +362,6 @@ __device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZ
         }
       }
     }
-    sums += kInt4Inputs / kGroup * kInt4MaxTiles * 8;
     ++tail;
     __syncwarp();                                    // the record is read: the copies run on into its stage
     int4_fetch<kGroup, kZeros>(a, sm, blocks, units, warp, lane, cursor);
@@ -528,18 +507,10 @@ int4_matvec_kernel(const Int4Args a) {
 #pragma unroll 1
   for (int i = 0; i < kInt4Stages; ++i) int4_fetch<kGroup, kZeros>(a, sm, blocks, units, warp, lane, cursor);
   pdl_wait();
-  int before = kInt4MaxLog, entry = -1;
+  int before = kInt4MaxLog;
   uint32_t tail = 0;
   do {
-    const bool wide = sm.entry_slots[item.entry] > 8;
-    if (item.entry != entry) {
-      entry = item.entry;
-      __syncthreads();                               // nobody reads the last entry's table any more
-      if (wide) int4_sums<T, 2, kGroup, kZeros>(a, sm, entry, units, warp, lane);
-      else int4_sums<T, 1, kGroup, kZeros>(a, sm, entry, units, warp, lane);
-      __syncthreads();
-    }
-    if (wide) int4_item<T, 2, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
+    if (sm.entry_slots[item.entry] > 8) int4_item<T, 2, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
     else int4_item<T, 1, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
   } while (item.next(a, blocks, units, warp));
 }
@@ -569,14 +540,11 @@ static int int4_launch(Int4Args a, int64_t slots, bool after, cudaStream_t strea
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return STK_ERR_LAUNCH;
   const auto kernel = int4_matvec_kernel<T, kGroup, kZeros>;
-  const auto bytes = [](int units) {
-    return sizeof(Int4Smem<kGroup, kZeros>) + static_cast<size_t>(units) * (kInt4Inputs / kGroup) * kInt4MaxTiles * 8 * sizeof(float);
-  };
-  constexpr int kMaxUnits = kInt4MaxGroups * kGroup / kInt4Inputs;
+  constexpr int kBytes = sizeof(Int4Smem<kGroup, kZeros>);
   if (sms[dev] == 0) {
     int n = 0;
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0 ||
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes(kMaxUnits))) != cudaSuccess) {
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) {
       cudaGetLastError();
       return STK_ERR_LAUNCH;
     }
@@ -589,9 +557,9 @@ static int int4_launch(Int4Args a, int64_t slots, bool after, cudaStream_t strea
     a.first_slot = static_cast<int>(first);
     a.slots = static_cast<int>(slots - first < kInt4MaxSlots ? slots - first : kInt4MaxSlots);
     if (after && first == 0)
-      launch_dependent(kernel, sms[dev], kInt4Threads, static_cast<int>(bytes(units)), stream, a);
+      launch_dependent(kernel, sms[dev], kInt4Threads, kBytes, stream, a);
     else
-      kernel<<<static_cast<unsigned>(sms[dev]), kInt4Threads, bytes(units), stream>>>(a);
+      kernel<<<static_cast<unsigned>(sms[dev]), kInt4Threads, kBytes, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return STK_ERR_LAUNCH;
   }
   return STK_OK;

@@ -273,3 +273,31 @@ def test_quantized_experts_stay_near_the_16_bit_ones():
     small = dmoe.expert_mlp_int4(x, ids, weights, dmoe.quantize_int4(w1.view(hidden, experts, ffn).transpose(0, 1)),
                                  dmoe.quantize_int4(w2.view(experts, ffn, hidden))).float()
     assert float((small - full).norm() / full.norm()) <= 0.3
+
+
+@pytest.mark.parametrize("tokens,inputs,group", [(3, 256, 128), (12, 192, 64), (16, 1024, 32), (1, 96, 32)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_inputs_under_zero_weights_add_nothing(tokens, inputs, group, zeros, dtype):
+    """Codes at the zero point stand for weights of 0: inputs of 3e4 under them leave a result within the tolerance above,
+    whose S does not know them, and a row of such codes gives exactly 0, whatever its scales are.  (0 times a finite
+    number is 0 in the products and aligns no other term.)  Inputs with a large mean have a large S and are within it."""
+    from stk_b200 import dmoe
+    outputs = 50
+    codes, _, scales, zero = bits(1, outputs, inputs, group, dtype, zeros, 11)
+    point = torch.full_like(codes, 8) if zero is None else zero.repeat_interleave(group, 2)
+    codes[:, :, ::7] = point[:, :, ::7]
+    nothing = [0, 3, 9, 21, 49]
+    codes[:, nothing] = point[:, nothing]
+    w = dmoe.pack_int4((codes[..., 0::2] | (codes[..., 1::2] << 4)).cuda(), scales.cuda(), None if zero is None else zero.cuda())
+    full = values(codes, scales, zero, group)[0]
+    g = torch.Generator().manual_seed(12)
+    x = torch.randn(tokens, inputs, generator=g)
+    outliers = x.clone()
+    outliers[:, ::7] = 3e4 * torch.sign(x[:, ::7])
+    for some in (outliers.to(dtype), (x + 200).to(dtype)):
+        y = dmoe.int4_matvec(some.cuda(), w).cpu().double()
+        assert not bool(y[:, nothing].any())
+        expect, size = some.double() @ full.t(), some.double().abs() @ full.abs().t()
+        tol = half_step(dtype) * expect.abs() + ((inputs / 32 + 16) * U32 + 2.0 ** -22) * size + TINY[dtype]
+        assert bool(((y - expect).abs() <= tol).all())
