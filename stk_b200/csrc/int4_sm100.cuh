@@ -199,8 +199,10 @@ __device__ __forceinline__ uint32_t int4_constant(uint32_t v) {
   return r;
 }
 
-// The products' epilogue's GeLU; a NaN stays one.
-__device__ __forceinline__ float int4_gelu(float x) { return x == x ? gelu_erf(x) : x; }
+// x Phi(x) = x erfc(-x / sqrt 2) / 2, for a few outputs each: to (x^2 + 8) 2^-23, relative, in the tail too (from the rounded
+// argument's x^2 2^-23 and erfcf's own error).  Below -16 it is beneath 32 bits, and -infinity gives -0 as in the products'
+// epilogues, whose shorter form has a constant tail below -8.  A NaN stays one.
+__device__ __forceinline__ float int4_gelu(float x) { return x < -16.0f ? -0.0f : 0.5f * x * erfcf(-0.70710678f * x); }
 
 __device__ __forceinline__ void int4_copy(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"

@@ -301,3 +301,23 @@ def test_inputs_under_zero_weights_add_nothing(tokens, inputs, group, zeros, dty
         expect, size = some.double() @ full.t(), some.double().abs() @ full.abs().t()
         tol = half_step(dtype) * expect.abs() + ((inputs / 32 + 16) * U32 + 2.0 ** -22) * size + TINY[dtype]
         assert bool(((y - expect).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_gelu_of_exact_products(dtype):
+    """One input under a weight of 1: the product is exact, and what remains is the GeLU's own error: (x^2 + 8) 2^-23 of it (its
+    argument is rounded twice, by 2^-24 each, which x^2 multiplies in the negative tail; erfc and two products add a few 2^-24), half a
+    step of the type, and half the type's smallest step."""
+    from stk_b200 import dmoe
+    v = torch.tensor([0.0, 1e-6, -1e-6, 1e-3, -1e-3, 0.05, -0.05, 0.5, -0.5, 1.0, -1.0, 2.5, -2.5, 4.0, -4.0, 5.8, -5.8, -6.5, -7.9, 8.0,
+                      -8.0, -8.1, -8.5, -9.0, -10.0, -12.0, -13.0, -14.0, -17.0, -100.0, -3e4, 12.0, 3e4]).to(dtype)
+    codes = torch.full((1, 32, 32), 8, dtype=torch.uint8)
+    codes[0, :, 5] = 9
+    w = dmoe.pack_int4((codes[..., 0::2] | (codes[..., 1::2] << 4)).cuda(), torch.ones(1, 32, 1, dtype=dtype, device="cuda"))
+    x = torch.zeros(len(v), 32, dtype=dtype)
+    x[:, 5] = v
+    y = dmoe.int4_matvec(x.cuda(), w, gelu=True).cpu().double()
+    exact = v.double()
+    expect = (0.5 * exact * torch.special.erfc(-exact * 0.5 ** 0.5))[:, None]
+    tol = (half_step(dtype) + (exact.clamp(max=0) ** 2 + 8)[:, None] * 2 * U32) * expect.abs() + TINY[dtype]
+    assert bool(((y - expect).abs() <= tol).all())
