@@ -11,8 +11,8 @@
 // bits, and that of the result: the error goes by sum |w x|, and an input whose code is the zero point adds exactly nothing.
 // (Summing (16 + code) x and taking (16 + zero) sum x away from the sum instead is cheaper by the subtractions and dearer by
 // a table of input sums, and its error goes by sum (32 + code + zero) |scale x|, which outliers among the inputs make
-// large.)  An infinity among the inputs makes its results infinite or NaN; so do finite ones whose sum of (code - zero) x
-// over a group is beyond the range of 32 bits (bf16 inputs above 1e35).
+// large.)  An infinity among the inputs makes its results infinite, or NaN where its weight is 0; so do finite ones whose sum
+// of (code - zero) x over a group is beyond the range of 32 bits (bf16 inputs above 1e35).
 //
 // Layout (made once, by the host): a record holds 32 output rows (two strips of 16) x 128 inputs, in the order in which
 // the kernel reads them.  First the codes, strip by strip, 64 inputs at a time, 512 bytes in the order in which the lanes
@@ -21,7 +21,7 @@
 // order of the inputs inside a product is free, so a lane's share of x is 16 contiguous bytes.)  A word is turned left by
 // 3 bits (bf16) or 6 (fp16), so that its first two codes lie where a 16-bit float has its last exact bits.  Then the
 // scales [group of the record][strip][g][r], then the zero points in the same order, a byte each.  What is beyond the
-// last row or input is code 0, scale 0, zero point 0: nothing.
+// last row or input is code 0, scale 0, zero point 0, and not added up.
 //
 // One CTA of 16 warps per SM takes an equal share of the records' rows (of every expert and tile of up to 16 of its
 // slots), several of them at a time: an item is 1, 2, 4, 8 or 16 of them, as many as are left, so that shares stay equal
@@ -265,8 +265,8 @@ struct Int4Inputs {
 #pragma unroll
     for (int n = 0; n < NT; ++n) x[n] += kInt4Inputs;
   }
-  // A quarter, of 32 inputs, of record c, which x is at.  (One beyond the inputs has codes, scales and zero points of 0:
-  // any of the row's values will do.  A choice between loaded values and zeros would wait for the load where it stands.)
+  // A quarter, of 32 inputs, of record c, which x is at.  (One beyond the inputs is not added up: any of the row's values
+  // will do.  A choice between loaded values and zeros would wait for the load where it stands.)
   __device__ __forceinline__ void load(const Int4Args& a, int c, int quarter, uint4 (&to)[NT]) const {
     const int at = kGroup == 128 || c * kInt4Inputs + quarter * 32 < a.inputs ? 4 * quarter : 0;
 #pragma unroll
@@ -353,7 +353,8 @@ __device__ __forceinline__ void int4_item(const Int4Args& a, Int4Smem<kGroup, kZ
       if (h == 4 - kAhead) in.next();
       if (h + kAhead < 4) in.load(a, c, h + kAhead, xq[h % kAhead]);
       else if (c + 1 < c1) in.load(a, c + 1, h + kAhead - 4, xq[h % kAhead]);
-      if (h % kPer == kPer - 1) {                    // the end of a group
+      // the end of a group (one beyond the inputs is left out: its x is another quarter's, and infinite if that is)
+      if (h % kPer == kPer - 1 && (kGroup == 128 || c * kInt4Inputs + h / kPer * kGroup < a.inputs)) {
 #pragma unroll
         for (int r = 0; r < kInt4Strips; ++r) {
           const float2 scale = Int4Type<T>::pair(st.scales[h / kPer][r][g]);

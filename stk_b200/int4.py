@@ -173,8 +173,8 @@ def int4_matvec(x, w, expert_ids=None, gelu=False):
     """y[t, j] = W_e x[t] for e = expert_ids[t, j]: [T, k, N] in x's type (sums in 32 bits, rounded once), zeros where
     the id is negative; without expert_ids (weights of one expert) [T, N].  gelu: the GeLU (erf form) of the products.
     x [T, K] float16 or bfloat16, the type of the weights' scales.  Weights are exact (code - zero) times their scale: what
-    lies under a code at its zero point adds nothing.  An infinity in a row of x makes its results infinite or NaN, and so may
-    finite values above 1e35 (a group's sum is taken before its scale).
+    lies under a code at its zero point adds nothing.  An infinity in a row of x makes its results infinite, or NaN where its weight
+    is 0, and so may finite values above 1e35 (a group's sum is taken before its scale).
     Made for few tokens: an expert's weights are read once for every 16 slots that chose it, and anew for every 256
     slots of the call."""
     _check_call("int4_matvec", x, w, expert_ids)

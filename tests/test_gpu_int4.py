@@ -321,3 +321,22 @@ def test_gelu_of_exact_products(dtype):
     expect = (0.5 * exact * torch.special.erfc(-exact * 0.5 ** 0.5))[:, None]
     tol = (half_step(dtype) + (exact.clamp(max=0) ** 2 + 8)[:, None] * 2 * U32) * expect.abs() + TINY[dtype]
     assert bool(((y - expect).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("inputs,group", [(32, 32), (64, 64), (160, 32), (192, 64), (128, 128)])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_infinite_inputs(inputs, group, zeros, dtype):
+    """An infinity goes into its results as the formula has it, also where a record of 128 inputs is not full."""
+    from stk_b200 import dmoe
+    codes = torch.full((1, 32, inputs // 2), 0x99, dtype=torch.uint8, device="cuda")
+    scales = torch.ones(1, 32, inputs // group, dtype=dtype, device="cuda")
+    w = dmoe.pack_int4(codes, scales, torch.full_like(scales, 8, dtype=torch.uint8) if zeros else None)
+    for at in (5, inputs - 32, inputs - 1):
+        x = torch.ones(4, inputs, dtype=dtype, device="cuda")
+        x[0, at], x[1, at], x[2, at] = torch.inf, -torch.inf, torch.nan
+        y = dmoe.int4_matvec(x, w)
+        assert bool((y[0] == torch.inf).all()) and bool((y[1] == -torch.inf).all()) and bool(y[2].isnan().all())
+        assert bool((y[3] == inputs).all())
+        y = dmoe.int4_matvec(x, w, gelu=True)
+        assert bool((y[0] == torch.inf).all()) and bool((y[1] == 0).all()) and bool(y[2].isnan().all())
