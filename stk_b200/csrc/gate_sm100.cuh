@@ -183,6 +183,7 @@ gate_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int expert
 
   const bool plain_softmax = !sigmoid_score && !normalize;
   float top = 0.0f, sum = 0.0f;  // the maximum, the denominator
+  int found = 0;                 // choices that have an expert
   for (int j = 0; j < k; ++j) {
     float best = -INFINITY;
     int at = 0;
@@ -203,6 +204,7 @@ gate_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int expert
       }
     }
     const bool taken = best > -INFINITY;
+    found += taken;
     if (j == 0) {
       top = taken ? best : 0.0f;
       if (plain_softmax) {
@@ -232,7 +234,7 @@ gate_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int expert
   __syncwarp();
   if (!here) return;
   if (sigmoid_score && !normalize) sum = 1.0f;
-  for (int j = lane; j < k; j += G) weights[t * k + j] = sum != 0.0f ? chosen[j] / sum + nan : 0.0f;
+  for (int j = lane; j < k; j += G) weights[t * k + j] = j < found ? chosen[j] / sum + nan : 0.0f;
   if (lane == 0 && stats != nullptr) stats[t] = make_float2(top, sum);
 }
 

@@ -457,3 +457,24 @@ def test_second_derivatives_are_refused():
     grad, = torch.autograd.grad((dmoe.sort_tokens(x, plan) ** 2).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         grad.sum().backward()
+
+
+@pytest.mark.parametrize("score,normalize", KINDS)
+def test_gate_choices_without_an_expert_weigh_nothing_beside_nan_and_infinity(score, normalize):
+    """Fewer than k logits above -inf, and one of them NaN or +inf: the choices that are left over have id -1 and weight 0, as
+    on the host, and every choice of a row with a NaN has weight NaN."""
+    from stk_b200 import dmoe
+    for dtype in DTYPES:
+        for experts in (3, 16, 40, 300):
+            logits = torch.full((6, experts), -torch.inf, dtype=dtype)
+            logits[0, 2], logits[1, 1] = torch.nan, torch.inf
+            logits[2, 0], logits[2, 2] = torch.nan, 1.0
+            logits[3, 0], logits[3, 2] = torch.inf, 1.0
+            logits[4, 2], logits[4, 1] = 2.0, 1.0
+            logits[5] = torch.nan
+            weights, ids = dmoe.top_k_gate(logits.cuda(), 3, score=score, normalize=normalize)
+            expect, expect_ids = dmoe.top_k_gate(logits, 3, score=score, normalize=normalize)
+            assert torch.equal(ids.cpu(), expect_ids)
+            torch.testing.assert_close(weights.cpu(), expect, rtol=128 * ref.U32, atol=0, equal_nan=True)
+            assert not bool(weights[ids < 0].any())
+            assert bool(weights[[0, 2, 5]][ids[[0, 2, 5]] >= 0].isnan().all())
