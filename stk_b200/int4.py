@@ -9,7 +9,7 @@ The reference has no counterpart.
 import torch
 
 from stk_b200.backend import lib as _lib
-from stk_b200.routing import ids32
+from stk_b200.routing import ids32, refuse_tangents
 
 GROUPS = (32, 64, 128)
 MAX_EXPERTS = 1024
@@ -149,6 +149,7 @@ def _check_call(what, x, w, expert_ids):
                                    expert_ids.dtype not in (torch.int16, torch.int32, torch.int64)):
         raise ValueError(f"{what}: expert_ids must be integers [{x.shape[0]}, k], got {expert_ids.dtype} "
                          f"{tuple(expert_ids.shape)}")
+    refuse_tangents(what, x)
     if not x.is_cuda:
         raise RuntimeError(f"{what} runs on CUDA tensors only (there is no CPU path); got a tensor on {x.device}")
     if w.device != x.device or (expert_ids is not None and expert_ids.device != x.device):
@@ -196,6 +197,7 @@ def expert_mlp_int4(x, expert_ids, weights, w1, w2):
     contributes nothing); w1, w2: Int4Experts with f outputs and f inputs.  The hidden activations are rounded to x's
     type, as in dmoe.expert_mlp; the sums over inputs and over choices are in 32 bits and rounded once."""
     _check_call("expert_mlp_int4", x, w1, expert_ids)
+    refuse_tangents("expert_mlp_int4", weights)
     if not isinstance(w2, Int4Experts) or w2.num_experts != w1.num_experts or w2.inputs != w1.outputs \
             or w2.dtype != w1.dtype or w2.device != w1.device:
         raise ValueError("expert_mlp_int4: w2 must hold the same experts, in the same type and on the same device, with "

@@ -12,12 +12,14 @@ A step with its backward pass can be captured in a CUDA graph (plan_tokens with 
 same leaves is alive that was made on the default stream: torch's engine waits for the stream of a leaf's accumulator,
 in torch.autograd.grad too, and raises an error where that is not the capturing one.
 
-On CUDA tensors everything runs as kernels of libstk_b200.so.  Host tensors take plain torch operations (as in
+On CUDA tensors everything runs as kernels of libstk_b200.so, with first derivatives in reverse mode; second ones and those
+in forward mode are refused.  Host tensors take plain torch operations (as in
 stk_b200.dmoe: for tests, not for production use).  The reference is a matmul library and has no counterpart.
 """
 import threading
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from stk_b200.backend import lib as _lib
@@ -43,6 +45,15 @@ def ids32(ids):
     if ids.dtype == torch.int64:
         ids = ids.clamp(-1, 2 ** 31 - 1)
     return ids.to(torch.int32).contiguous()
+
+
+def refuse_tangents(what, *tensors):
+    """The kernels have no forward-mode derivatives, and a tangent that they dropped would count as zero."""
+    if forward_ad._current_level < 0:                  # outside every dual level nothing has one (0.8 us of 10 to ask a call's)
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what} has no forward-mode derivative")
 
 
 def _once(backward):
@@ -145,6 +156,7 @@ def top_k_gate(logits, top_k, score="softmax", normalize=True, token_mask=None):
         token_mask = token_mask.contiguous()
     if not logits.is_cuda:
         return _host_gate(logits, token_mask, top_k, _SCORES[score], normalize)
+    refuse_tangents("top_k_gate", logits)
     args = (logits, token_mask, int(top_k), _SCORES[score], int(bool(normalize)))
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TopKGate.apply(*args)
@@ -325,6 +337,7 @@ def sort_tokens(x, plan):
     32 bits."""
     _check_rows("sort_tokens", x, plan.tokens, "tokens of the plan", plan)
     if x.is_cuda:
+        refuse_tangents("sort_tokens", x)
         return _SortTokens.apply(x, plan) if torch.is_grad_enabled() and x.requires_grad else _sort_rows(x, plan)
     valid = plan.index >= 0
     out = x.new_zeros((plan.rows, x.shape[1]))
@@ -348,6 +361,7 @@ def unsort_tokens(rows, weights, plan):
             weights = weights[:, None]
         weights = weights.float().contiguous()
     if rows.is_cuda:
+        refuse_tangents("unsort_tokens", rows, weights)
         if torch.is_grad_enabled() and (rows.requires_grad or (weights is not None and weights.requires_grad)):
             return _UnsortTokens.apply(rows, weights, plan)
         return _sum_rows(rows, weights, plan)

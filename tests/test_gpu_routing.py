@@ -478,3 +478,29 @@ def test_gate_choices_without_an_expert_weigh_nothing_beside_nan_and_infinity(sc
             torch.testing.assert_close(weights.cpu(), expect, rtol=128 * ref.U32, atol=0, equal_nan=True)
             assert not bool(weights[ids < 0].any())
             assert bool(weights[[0, 2, 5]][ids[[0, 2, 5]] >= 0].isnan().all())
+
+
+def test_tangents_are_refused():
+    """Forward-mode differentiation: the kernels refuse a dual tensor, with and without a graph, instead of dropping its
+    tangent, and take the same tensors without one inside a dual level."""
+    from torch.autograd import forward_ad
+    from stk_b200 import dmoe
+    plan = dmoe.plan_tokens(torch.tensor([[0, 1], [1, 2]], device="cuda"), 3)
+    x, logits = torch.randn(2, 8, device="cuda"), torch.randn(2, 3, device="cuda")
+    rows, weights = torch.randn(plan.rows, 8, device="cuda"), torch.rand(2, 2, device="cuda")
+    w = dmoe.quantize_int4(torch.randn(3, 32, 32, device="cuda").half(), group=32)
+    h, ids = torch.randn(2, 32, device="cuda").half(), torch.zeros(2, 2, dtype=torch.int32, device="cuda")
+    calls = [lambda d: dmoe.top_k_gate(d(logits), 2), lambda d: dmoe.sort_tokens(d(x), plan),
+             lambda d: dmoe.unsort_tokens(d(rows), weights, plan), lambda d: dmoe.unsort_tokens(rows, d(weights), plan),
+             lambda d: dmoe.int4_matvec(d(h), w, ids), lambda d: dmoe.expert_mlp_int4(d(h), ids, weights, w, w),
+             lambda d: dmoe.expert_mlp_int4(h, ids, d(weights), w, w)]
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in calls:
+            call(lambda t: t)
+            for context in (torch.enable_grad, torch.no_grad):
+                with context(), pytest.raises(RuntimeError, match="forward-mode"):
+                    call(dual)
+        leaf = x.clone().requires_grad_()
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            dmoe.sort_tokens(dual(leaf), plan)

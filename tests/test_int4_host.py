@@ -115,3 +115,20 @@ def test_entry_points_check_before_any_launch():
     assert mlp(weights=None) == -1 and mlp(ws=None) == -7 and mlp(ws=p + 4) == -7 and mlp(size=8191) == -7
     assert mlp(dtype=3) == -3 and mlp(tokens=1 << 31) == -9
     assert L.stk_b200_int4_mlp_workspace_bytes(8, 256, 128) == 8192 and L.stk_b200_int4_mlp_workspace_bytes(0, 256, 128) == 0
+
+
+def test_tangents_are_refused_before_any_launch():
+    """A dual tensor of forward-mode differentiation requires no gradient; its tangent must not be dropped without a word."""
+    from torch.autograd import forward_ad
+    from stk_b200 import dmoe
+    w = dmoe.quantize_int4(torch.randn(2, 64, 64).half(), group=64)
+    x, ids, weights = torch.randn(3, 64).half(), torch.zeros(3, 2, dtype=torch.int32), torch.ones(3, 2)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: dmoe.int4_matvec(dual, w, ids), lambda: dmoe.expert_mlp_int4(dual, ids, weights, w, w)):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+        with pytest.raises(RuntimeError, match="CUDA tensors only"):
+            dmoe.int4_matvec(x, w, ids)                   # (no tangent: the next check's)
+    with pytest.raises(RuntimeError, match="CUDA tensors only"):
+        dmoe.int4_matvec(x, w, ids)

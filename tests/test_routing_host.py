@@ -134,3 +134,24 @@ def test_entry_points_check_before_any_launch():
     assert L.stk_b200_sum_rows(p, 8, p, None, p, 4, 2, 0, 1, None) == 0
     assert L.stk_b200_unsort_backward(p, 8, p, 8, p, None, p, p, None, 4, 2, 128, 8, 1, None) == -1
     assert L.stk_b200_unsort_backward(p, 8, p, 8, p, p, p, None, None, 4, 2, 128, 8, 1, None) == 0
+
+
+def test_tangents_go_through_the_host_path():
+    """Host tensors take torch operations, which have forward-mode derivatives: they agree with the reverse mode's."""
+    from torch.autograd import forward_ad
+    from stk_b200 import dmoe
+    g = torch.Generator().manual_seed(4)
+    plan = dmoe.plan_tokens(torch.tensor([[0, 2], [1, -1], [2, 1], [0, 1]]), 3)
+    x, dx = torch.randn(4, 5, generator=g), torch.randn(4, 5, generator=g)
+    logits, dlogits = torch.randn(4, 6, generator=g), torch.randn(4, 6, generator=g)
+
+    def value(x, logits):
+        weights, _ = dmoe.top_k_gate(logits, 2, normalize=False)
+        return dmoe.unsort_tokens(dmoe.sort_tokens(x, plan), weights, plan).square().sum()
+
+    leaves = [x.clone().requires_grad_(), logits.clone().requires_grad_()]
+    grads = torch.autograd.grad(value(*leaves), leaves)
+    with forward_ad.dual_level():
+        out = value(forward_ad.make_dual(x, dx), forward_ad.make_dual(logits, dlogits))
+        slope = forward_ad.unpack_dual(out).tangent
+    torch.testing.assert_close(slope, (grads[0] * dx).sum() + (grads[1] * dlogits).sum(), rtol=1e-4, atol=1e-5)
