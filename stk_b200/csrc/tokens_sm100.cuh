@@ -32,6 +32,9 @@ __device__ __forceinline__ int slot_expert(const int32_t* ids, int64_t s, int64_
   return e < experts ? e : -1;
 }
 
+// Blocks of `n` slots.  (n + block - 1 may be beyond 32 bits where the rows are not.)
+__device__ __forceinline__ int32_t blocks_of(int32_t n, int block) { return n > 0 ? (n - 1) / block + 1 : 0; }
+
 // hist[g * experts + e] = slots of CTA g's share that chose expert e.
 __global__ void __launch_bounds__(kPlaceThreads)
 place_count_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int32_t* __restrict__ hist) {
@@ -109,7 +112,7 @@ place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int bl
     int32_t sum = 0;
     for (int i = 0; i < per; ++i) {
       const int e = lane * per + i;
-      if (e < experts) sum += (count[e] + block - 1) / block;
+      if (e < experts) sum += blocks_of(count[e], block);
     }
     int32_t up = sum;
 #pragma unroll
@@ -122,7 +125,7 @@ place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int bl
       const int e = lane * per + i;
       if (e < experts) {
         bin[e] = run * block;
-        run += (count[e] + block - 1) / block;
+        run += blocks_of(count[e], block);
       }
     }
     if (lane == 31) bin[experts] = up * block;
@@ -159,7 +162,7 @@ place_kernel(const int32_t* __restrict__ ids, int64_t slots, int experts, int bl
   // padding: the end of every bin, the experts dealt out to the warps of the grid; then what is left of `index`
   const int64_t warps = static_cast<int64_t>(gridDim.x) * kPlaceWarps;
   for (int64_t e = static_cast<int64_t>(blockIdx.x) * kPlaceWarps + warp; e < experts; e += warps)
-    for (int r = bin[e] + count[e] + lane; r < bin[e + 1]; r += 32) index[r] = -1;
+    for (int64_t r = static_cast<int64_t>(bin[e]) + count[e] + lane; r < bin[e + 1]; r += 32) index[r] = -1;
   for (int64_t r = used + static_cast<int64_t>(blockIdx.x) * kPlaceThreads + threadIdx.x; r < rows; r += warps * 32)
     index[r] = -1;
 }

@@ -504,3 +504,17 @@ def test_tangents_are_refused():
         leaf = x.clone().requires_grad_()
         with pytest.raises(RuntimeError, match="forward-mode"):
             dmoe.sort_tokens(dual(leaf), plan)
+
+
+def test_plan_with_bins_that_end_at_the_32_bit_limit():
+    """One bin whose last row is 2^31 - 2: neither slots + block - 1 nor the walk over the padding fits 32 bits."""
+    from stk_b200 import dmoe
+    for block, ids in ((2 ** 31 - 1, [0, 0]), (2 ** 31 - 16, [0, -1, 0])):
+        assert dmoe.plan_rows(len(ids), 1, block) == block
+        for rows in (None, block):
+            plan = dmoe.plan_tokens(torch.tensor(ids, device="cuda"), 1, block=block, rows=rows)
+            assert plan.rows == block and plan.block_rows == 1 and plan.bin_rows.tolist() == [1]
+            assert plan.position.tolist() == [i - (i > 0 and ids[1] < 0) if e >= 0 else -1 for i, e in enumerate(ids)]
+            assert plan.index[:4].tolist() == [s for s, e in enumerate(ids) if e >= 0] + [-1, -1]
+            assert bool((plan.index[2:] == -1).all())
+            del plan
