@@ -279,6 +279,14 @@ __device__ __noinline__ bool int4_wait(uint32_t bar, uint32_t parity, volatile i
   return mbar_wait(bar, parity, stuck);
 }
 
+// After a wait has run out: the warp's last copies, which may still land in its ring, are waited for, with a limit as well, so
+// that the block's shared memory is not handed on while they do.  head: how many it has started.
+__device__ __noinline__ void int4_drain(uint32_t bars, uint32_t head) {
+  volatile int given_up = 0;
+  for (uint32_t i = head > kInt4Stages ? head - kInt4Stages : 0; i < head; ++i)
+    mbar_wait(bars + 8 * (i % kInt4Stages), i / kInt4Stages & 1u, &given_up);
+}
+
 // The warp's part of an item: records [c0, c1), from the ring's stage tail % kInt4Stages on; NT tiles of 8 slots.
 // before: the last item's log.
 template <typename T, int NT, int kGroup, bool kZeros>
@@ -516,6 +524,7 @@ int4_matvec_kernel(const Int4Args a) {
     if (sm.entry_slots[item.entry] > 8) int4_item<T, 2, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
     else int4_item<T, 1, kGroup, kZeros>(a, sm, item, blocks, units, warp, lane, tail, before, cursor);
   } while (item.next(a, blocks, units, warp));
+  if (*static_cast<volatile int*>(&sm.stuck) != 0) int4_drain(smem_u32(&sm.full[warp][0]), cursor.head);
 }
 
 // out[t] = sum_j weights[t, j] * y[t * k + j] over the choices that have an expert; y in 32 bits.

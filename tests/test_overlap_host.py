@@ -47,3 +47,14 @@ def test_the_second_4_bit_product_reads_its_inputs_so():
     _, body = kernel(text, "int4_matvec_kernel")
     wait = body.rindex("pdl_wait()")
     assert all(m.start() > wait for m in re.finditer(r"int4_(item|sums)<", body))
+
+
+def test_a_block_that_gives_up_a_wait_waits_for_its_copies():
+    """A bulk copy that lands after its block has ended would write into another block's shared memory.  (No test makes a
+    copy late: the sources show the wait, after the items, for what each warp has started.)"""
+    text = source("int4_sm100.cuh")
+    _, body = kernel(text, "int4_matvec_kernel")
+    end = body[body.rindex("while (item.next("):]
+    assert re.search(r"if \(\*static_cast<volatile int\*>\(&sm\.stuck\) != 0\) int4_drain\([^;]*cursor\.head\);", end)
+    drain = text[text.index("void int4_drain("):]
+    assert "mbar_wait(" in drain[:drain.index("\n}\n")]
