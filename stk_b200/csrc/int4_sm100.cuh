@@ -588,9 +588,8 @@ static int int4_by_group(const Int4Args& a, int group, int zeros, int64_t slots,
   return int4_launch<T, 128, true>(a, slots, after, stream);
 }
 
-static int int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots, int x_div,
-                       int experts, int64_t outputs, int64_t inputs, int group, int zeros, int gelu, int out_f32,
-                       int dtype, bool after, cudaStream_t stream) {
+static int int4_check(const void* records, const void* x, const int32_t* ids, const void* out, int64_t slots, int x_div,
+                      int experts, int64_t outputs, int64_t inputs, int group, int dtype) {
   if (slots < 0 || x_div < 1 || experts < 1 || outputs < 1 || inputs < 1) return STK_ERR_BAD_DIMS;
   if ((group != 32 && group != 64 && group != 128) || inputs % group) return STK_ERR_BAD_DIMS;
   if (dtype != STK_F16 && dtype != STK_BF16) return STK_ERR_BAD_DTYPE;
@@ -599,6 +598,13 @@ static int int4_matvec(const void* records, const void* x, const int32_t* ids, v
   if (slots == 0) return STK_OK;
   if (!records || !x || !ids || !out) return STK_ERR_NULL_POINTER;
   if ((reinterpret_cast<uintptr_t>(records) | reinterpret_cast<uintptr_t>(x)) % 16) return STK_ERR_BAD_LAYOUT;
+  return STK_OK;
+}
+static int int4_matvec(const void* records, const void* x, const int32_t* ids, void* out, int64_t slots, int x_div,
+                       int experts, int64_t outputs, int64_t inputs, int group, int zeros, int gelu, int out_f32,
+                       int dtype, bool after, cudaStream_t stream) {
+  const int rc = int4_check(records, x, ids, out, slots, x_div, experts, outputs, inputs, group, dtype);
+  if (rc != STK_OK || slots == 0) return rc;
   const Int4Args a{static_cast<const unsigned char*>(records), x, ids, out, 0, 0, x_div, experts,
                    static_cast<int>(outputs), static_cast<int>(inputs), 0, gelu, out_f32};
   return dtype == STK_BF16 ? int4_by_group<__nv_bfloat16>(a, group, zeros, slots, after, stream)
@@ -634,15 +640,19 @@ extern "C" int stk_b200_int4_mlp(const void* records1, const void* records2, con
   if (tokens < 0 || top_k < 1 || outputs < 1 || ffn < 1) return STK_ERR_BAD_DIMS;
   if (tokens == 0) return STK_OK;
   if (!weights || !out) return STK_ERR_NULL_POINTER;
-  if (tokens > INT32_MAX / top_k) return STK_ERR_TOO_LARGE;
+  if (tokens > INT32_MAX / top_k || outputs > (1 << 20) || ffn > (1 << 20)) return STK_ERR_TOO_LARGE;
   const int64_t slots = tokens * top_k, blocks = (tokens * outputs + 255) / 256;
-  if (blocks > INT32_MAX || ffn > (1 << 20)) return STK_ERR_TOO_LARGE;
+  if (blocks > INT32_MAX) return STK_ERR_TOO_LARGE;
   if (workspace == nullptr || reinterpret_cast<uintptr_t>(workspace) % 16 ||
       workspace_bytes < stk_b200_int4_mlp_workspace_bytes(slots, ffn, outputs))
     return STK_ERR_WORKSPACE;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  // both products' arguments before the first one runs
+  int rc = stk::int4_check(records1, x, ids, workspace, slots, top_k, experts, ffn, hidden, group1, dtype);
+  if (rc == STK_OK) rc = stk::int4_check(records2, workspace, ids, workspace, slots, 1, experts, outputs, ffn, group2, dtype);
+  if (rc != STK_OK) return rc;
   float* y = reinterpret_cast<float*>(static_cast<unsigned char*>(workspace) + stk::int4_hidden_bytes(slots, ffn));
-  int rc = stk::int4_matvec(records1, x, ids, workspace, slots, top_k, experts, ffn, hidden, group1, zeros1, 1, 0, dtype, false, s);
+  rc = stk::int4_matvec(records1, x, ids, workspace, slots, top_k, experts, ffn, hidden, group1, zeros1, 1, 0, dtype, false, s);
   if (rc != STK_OK) return rc;
   rc = stk::int4_matvec(records2, workspace, ids, y, slots, 1, experts, outputs, ffn, group2, zeros2, 0, 1, dtype, true, s);
   if (rc != STK_OK) return rc;

@@ -132,3 +132,14 @@ def test_tangents_are_refused_before_any_launch():
             dmoe.int4_matvec(x, w, ids)                   # (no tangent: the next check's)
     with pytest.raises(RuntimeError, match="CUDA tensors only"):
         dmoe.int4_matvec(x, w, ids)
+
+
+def test_the_mlp_checks_its_second_product_before_the_first_one_runs():
+    """Without a device a launch fails with another code than these."""
+    from stk_b200.backend import lib
+    L = lib.load()
+    p = 4096                                              # an aligned address that is never read
+    mlp = lambda second=p, outputs=128, ffn=256, group=64: L.stk_b200_int4_mlp(
+        p, second, p, p, p, p, 4, 2, 2, 128, ffn, outputs, 64, 0, group, 0, 1, p, 1 << 40, None)
+    assert mlp(group=48) == -2 and mlp(group=64, ffn=96) == -2 and mlp(second=None) == -1 and mlp(second=p + 8) == -4
+    assert mlp(outputs=(1 << 20) + 32) == -9 and mlp(ffn=513 * 64) == -9
