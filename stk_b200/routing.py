@@ -40,6 +40,13 @@ def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else max(t.shape[1], 1)
 
 
+def _whole(what, name, value):
+    n = int(value)
+    if n != value:
+        raise ValueError(f"{what}: {name} must be a whole number, got {value}")
+    return n
+
+
 def ids32(ids):
     """Expert ids as contiguous int32; 64-bit ones beyond it stay beyond every expert."""
     if ids.dtype == torch.int64:
@@ -144,6 +151,7 @@ def top_k_gate(logits, top_k, score="softmax", normalize=True, token_mask=None):
         raise ValueError(f"top_k_gate: score must be one of {sorted(_SCORES)}, got {score!r}")
     tokens, experts = logits.shape
     _lib.row_dtype_code(logits.dtype)
+    top_k = _whole("top_k_gate", "top_k", top_k)
     if not 1 <= experts <= MAX_EXPERTS or not 1 <= top_k <= min(experts, MAX_TOP_K):
         raise ValueError(f"top_k_gate: 1 <= top_k <= min(experts, {MAX_TOP_K}) and experts <= {MAX_EXPERTS}, got "
                          f"top_k = {top_k}, {experts} experts")
@@ -157,7 +165,7 @@ def top_k_gate(logits, top_k, score="softmax", normalize=True, token_mask=None):
     if not logits.is_cuda:
         return _host_gate(logits, token_mask, top_k, _SCORES[score], normalize)
     refuse_tangents("top_k_gate", logits)
-    args = (logits, token_mask, int(top_k), _SCORES[score], int(bool(normalize)))
+    args = (logits, token_mask, top_k, _SCORES[score], int(bool(normalize)))
     if torch.is_grad_enabled() and logits.requires_grad:
         return _TopKGate.apply(*args)
     return _gate(*args, None)
@@ -207,11 +215,12 @@ def plan_tokens(expert_ids, num_experts, block=BLOCK, rows=None):
     if expert_ids.dim() not in (1, 2) or expert_ids.dtype not in (torch.int16, torch.int32, torch.int64):
         raise ValueError(f"plan_tokens: expert_ids must be integers [T] or [T, k], got {expert_ids.dtype} "
                          f"{tuple(expert_ids.shape)}")
+    num_experts, block = _whole("plan_tokens", "num_experts", num_experts), _whole("plan_tokens", "block", block)
+    rows = None if rows is None else _whole("plan_tokens", "rows", rows)
     if not 1 <= num_experts <= MAX_EXPERTS:
         raise ValueError(f"plan_tokens: 1 to {MAX_EXPERTS} experts, got {num_experts}")
     if block < 1:
         raise ValueError(f"plan_tokens: block must be positive, got {block}")
-    num_experts, block, rows = int(num_experts), int(block), None if rows is None else int(rows)
     tokens = expert_ids.shape[0]
     top_k = 1 if expert_ids.dim() == 1 else expert_ids.shape[1]
     if top_k < 1:

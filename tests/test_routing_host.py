@@ -155,3 +155,15 @@ def test_tangents_go_through_the_host_path():
         out = value(forward_ad.make_dual(x, dx), forward_ad.make_dual(logits, dlogits))
         slope = forward_ad.unpack_dual(out).tangent
     torch.testing.assert_close(slope, (grads[0] * dx).sum() + (grads[1] * dlogits).sum(), rtol=1e-4, atol=1e-5)
+
+
+def test_counts_are_whole_numbers():
+    """1.5 choices are not one choice."""
+    from stk_b200 import dmoe
+    x, ids = torch.randn(4, 8), torch.zeros(4, dtype=torch.int32)
+    for bad in (lambda: dmoe.top_k_gate(x, 1.5), lambda: dmoe.plan_tokens(ids, 4.5), lambda: dmoe.plan_tokens(ids, 4, block=16.5),
+                lambda: dmoe.plan_tokens(ids, 4, rows=512.5)):
+        with pytest.raises(ValueError, match="whole number"):
+            bad()
+    assert all(torch.equal(a, b) for a, b in zip(dmoe.top_k_gate(x, 2.0), dmoe.top_k_gate(x, 2)))
+    assert dmoe.plan_tokens(ids, 4.0, block=128.0, rows=512.0).rows == 512
