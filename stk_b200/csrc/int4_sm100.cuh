@@ -40,6 +40,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/stk_b200.h"
 #include "bsmm_sm100.cuh"
 #include "gate_sm100.cuh"
@@ -548,13 +550,13 @@ int4_combine_kernel(const float* y, const int32_t* __restrict__ ids, const float
 
 template <typename T, int kGroup, bool kZeros>
 static int int4_launch(Int4Args a, int64_t slots, bool after, cudaStream_t stream) {  // after: programmatic dependent launch
-  static int sms[64] = {};
+  static std::atomic<int> sms[64] = {};              // (two threads may fill it at once)
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return STK_ERR_LAUNCH;
   const auto kernel = int4_matvec_kernel<T, kGroup, kZeros>;
   constexpr int kBytes = sizeof(Int4Smem<kGroup, kZeros>);
-  if (sms[dev] == 0) {
-    int n = 0;
+  int n = sms[dev];
+  if (n == 0) {
     if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0 ||
         cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes) != cudaSuccess) {
       cudaGetLastError();
@@ -569,9 +571,9 @@ static int int4_launch(Int4Args a, int64_t slots, bool after, cudaStream_t strea
     a.first_slot = static_cast<int>(first);
     a.slots = static_cast<int>(slots - first < kInt4MaxSlots ? slots - first : kInt4MaxSlots);
     if (after && first == 0)
-      launch_dependent(kernel, sms[dev], kInt4Threads, kBytes, stream, a);
+      launch_dependent(kernel, n, kInt4Threads, kBytes, stream, a);
     else
-      kernel<<<static_cast<unsigned>(sms[dev]), kInt4Threads, kBytes, stream>>>(a);
+      kernel<<<static_cast<unsigned>(n), kInt4Threads, kBytes, stream>>>(a);
     if (cudaGetLastError() != cudaSuccess) return STK_ERR_LAUNCH;
   }
   return STK_OK;

@@ -340,3 +340,35 @@ def test_infinite_inputs(inputs, group, zeros, dtype):
         assert bool((y[3] == inputs).all())
         y = dmoe.int4_matvec(x, w, gelu=True)
         assert bool((y[0] == torch.inf).all()) and bool((y[1] == 0).all()) and bool(y[2].isnan().all())
+
+
+def test_first_calls_of_two_threads_at_once():
+    """Each kernel's first launch looks its device up; two threads may do so at the same time."""
+    import threading
+    from stk_b200 import dmoe
+    cases, wrong = [], []
+    for seed, (group, zeros, dtype) in enumerate([(32, True, torch.float16), (64, False, torch.bfloat16), (128, True, torch.bfloat16)]):
+        _, packed, scales, zero = bits(3, 96, 256, group, dtype, zeros, seed)
+        w = dmoe.pack_int4(packed, scales, zero).to("cuda")
+        g = torch.Generator().manual_seed(seed)
+        cases.append((torch.randn(5, 256, generator=g).to(dtype).cuda(), w, torch.randint(-1, 3, (5, 2), generator=g).cuda()))
+    start = threading.Barrier(2)
+
+    def work(out):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(20):
+                    out.append([dmoe.int4_matvec(*c) for c in cases])
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:  # noqa: BLE001
+            wrong.append(e)
+
+    torch.cuda.synchronize()
+    results = [[], []]
+    threads = [threading.Thread(target=work, args=(r,)) for r in results]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not wrong
+    alone = [dmoe.int4_matvec(*c) for c in cases]
+    assert all(torch.equal(a, b) for r in results for turn in r for a, b in zip(turn, alone))
