@@ -733,9 +733,10 @@ class _ExpertMLP(torch.autograd.Function):
         nnz = row_indices.numel()
         pre = torch.empty((nnz, BLOCK, BLOCK), dtype=x.dtype, device=x.device)
         act = torch.empty_like(pre)
-        _kernels.sdd(x, w1, shape, pre, offsets, row_indices, column_indices, epilogue=2, aux=act)
         y = torch.empty((shape[0], w2.shape[1]), dtype=x.dtype, device=x.device)
-        _kernels.dsd(shape, act, *meta, False, w2, y)
+        if shape[0]:                                        # (a batch may have no row: the products want some)
+            _kernels.sdd(x, w1, shape, pre, offsets, row_indices, column_indices, epilogue=2, aux=act)
+            _kernels.dsd(shape, act, *meta, False, w2, y)
         ctx.save_for_backward(x, w1, w2, pre, act, *meta)
         ctx.shape = tuple(shape)
         return y
@@ -746,6 +747,9 @@ class _ExpertMLP(torch.autograd.Function):
         meta = ctx.saved_tensors[5:]
         offsets, row_indices, column_indices = meta[:3]
         shape = ctx.shape
+        if not shape[0]:
+            return tuple(torch.zeros_like(t) if need else None
+                         for t, need in zip((x, w1, w2), ctx.needs_input_grad)) + (None,) * 7
         dy = dy.contiguous()
         dx = dw1 = dw2 = None
         if ctx.needs_input_grad[2]:
@@ -767,7 +771,7 @@ def expert_mlp(x, w1, w2, topo):
     """The experts' two-layer MLP of a dMoE layer on tokens in padded expert order:
     y = dsd(GeLU(sdd(x, w1, topo)), w2), differentiable in x, w1 and w2, with GeLU and its
     backward fused into the block-sparse products (see _ExpertMLP).  x [T', h], w1 [h, E*f],
-    w2 [E*f, h_out] on the GPU, fp16 or bf16; topo: the block-diagonal topology of the batch."""
+    w2 [E*f, h_out] on the GPU, fp16 or bf16; topo: the block-diagonal topology of the batch (which may have no row)."""
     assert isinstance(topo, Matrix) and topo.is_contiguous()
     return _ExpertMLP.apply(x.contiguous(), w1, w2, tuple(topo.size()), topo.offsets, topo.row_indices,
                             topo.column_indices, topo.offsets_t, topo.column_indices_t, topo.block_offsets_t)

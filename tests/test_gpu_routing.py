@@ -518,3 +518,22 @@ def test_plan_with_bins_that_end_at_the_32_bit_limit():
             assert plan.index[:4].tolist() == [s for s, e in enumerate(ids) if e >= 0] + [-1, -1]
             assert bool((plan.index[2:] == -1).all())
             del plan
+
+
+@pytest.mark.parametrize("tokens", [0, 6])
+@pytest.mark.parametrize("fixed", [False, True])
+def test_a_layer_on_a_batch_without_live_tokens(tokens, fixed):
+    """No tokens, or padding alone: the step runs, its output and its gradients are zeros of their shapes."""
+    from stk_b200 import dmoe
+    hidden, ffn, experts = 128, 256, 4
+    x, router, w1, w2 = (t.cuda().requires_grad_() for t in layer_inputs(tokens, hidden, ffn, experts, torch.float16))
+    mask = torch.zeros(tokens, dtype=torch.bool, device="cuda")
+    weights, ids = dmoe.top_k_gate(x @ router, 2, token_mask=mask)
+    plan = dmoe.plan_tokens(ids, experts, rows=512 if fixed else None)
+    assert plan.rows == (512 if fixed else 0)
+    topo = dmoe.topology_from_bins(plan.bin_rows, plan.block_rows, ffn, x.dtype, x.device, materialize=False)
+    y = dmoe.expert_mlp(dmoe.sort_tokens(x, plan), w1, w2, topo)
+    out = dmoe.unsort_tokens(y, weights, plan)
+    assert out.shape == (tokens, hidden) and not bool(out.any())
+    for leaf, grad in zip((x, router, w1, w2), torch.autograd.grad(out.float().sum(), (x, router, w1, w2))):
+        assert grad.shape == leaf.shape and not bool(grad.any())
