@@ -144,8 +144,9 @@ __device__ __forceinline__ float gate_exp(float d) {
 // G lanes per token, V logits per lane.  k rounds, each finding the largest remaining (value, lowest index) in
 // the lane's registers and then across the lanes by butterfly shuffles; what is chosen becomes -inf.
 // stats (optional): the row's maximum and sum, for the backward pass of the plain softmax.
-// Bound by its arithmetic (about 250 instructions a lane for 64 experts, 2 choices): 13 us for 131072 x 64 fp32 logits and
-// k = 2 (34 MB, 5 us of HBM time), 29 us for bf16 and k = 8.  Few lanes with many logits each, since a shuffle step
+// 13 us for 131072 x 64 fp32 logits and k = 2 (34 MB, 5 us of HBM time), 29 us for bf16 and k = 8.  Neither memory (26 % of
+// nominal) nor the SMs (48 %) are full: a block loads its logits and then goes through k dependent rounds, about 250
+// instructions a lane for 64 experts and 2 choices, with no load beside them, and its last wave is part full.  Few lanes with many logits each, since a shuffle step
 // costs as much as three logits: 16 logits a lane 18 us where 8 took 25 (k = 2, events and launch included).
 template <typename T, int G, int V, bool kVec>
 __global__ void __launch_bounds__(kGateThreads)

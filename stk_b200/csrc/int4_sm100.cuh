@@ -29,10 +29,12 @@
 // order.  Each warp streams its records through a ring of its own, by bulk copies that one lane starts; the copies run
 // ahead across the items.
 //
-// 32 slots on 8 experts of 4096 inputs x 14336 outputs, bf16, group 128 (242 MB, 37 us of HBM time): 58 - 62 us, of which the
-// copies alone take 41 and the arithmetic alone 49.  The arithmetic is 16.5 instructions for a word of 8 codes a lane,
-// 9.4 of them on the integer pipe.  Measured and no better: two rows of records per warp sharing their loads of x, 24
-// warps of 80 registers, a ring of 4, shifts by multiplication.
+// 32 slots on 8 experts of 4096 inputs x 14336 outputs, bf16, group 128 (242 MB, 37 us of HBM time): 64 - 70 us; the copies
+// alone take 41.  20.6 instructions for a word of 8 codes a lane, 9.5 of them on the integer pipe (59 % busy) and 4 the
+// subtractions (58 - 62 us with a table of input sums in their place, which is not exact); 0.64 instructions a clock and scheduler,
+// mma.sync 25 % busy: no one unit is full, the schedulers and the integer pipe together are nearest to it.  Measured and no
+// better: two rows of records per warp sharing their loads of x, 24 warps of 80 registers, a ring of 4, shifts by
+// multiplication, the subtraction as a packed multiply-add.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -613,7 +615,12 @@ static int int4_matvec(const void* records, const void* x, const int32_t* ids, v
                            : int4_by_group<__half>(a, group, zeros, slots, after, stream);
 }
 
-// Where the hidden activations and the second products lie in the workspace of int4_mlp.
+// Where the hidden activations and the second products lie in the workspace of int4_mlp.  The activations are rounded to the
+// inputs' type, as dmoe.expert_mlp's are: they are the B operand of the second product, and as pairs of 16-bit numbers,
+// which would keep 32 bits of them nearly whole, they would be twice the columns (2048 x 8192, 16 experts: 61 us with about
+// twice the columns where 43 without).  What it costs: the output's error against 64 bits is 1.70e-3 of its norm with and
+// without this rounding for 16 tokens of 4096 x 14336 (bf16; the output's own rounding is nearly all of it), and 1.82e-3
+// instead of 1.66e-3 for 64 tokens of 2048 x 8192 in groups of 64 with zero points, the largest seen.
 static size_t int4_hidden_bytes(int64_t slots, int64_t ffn) { return (static_cast<size_t>(slots) * ffn * 2 + 255) / 256 * 256; }
 
 }  // namespace stk

@@ -243,7 +243,8 @@ def route_top1(expert_ids, num_experts, block=BLOCK):
 
 def permute_tokens(x, index, total_rows=None, top_k=1):
     """Padded, expert-ordered copy of the token matrix x [T, h] (padding rows are zero); with top_k > 1
-    `index` holds slots and every token's row is copied to each of its k places."""
+    `index` holds slots and every token's row is copied to each of its k places.  Forward only, no gradient is
+    recorded: in training use plan_tokens / sort_tokens / unsort_tokens."""
     return gather_rows(x, index, total_rows, index_div=top_k)
 
 
@@ -253,7 +254,8 @@ def unpermute_tokens(y, index, tokens):
 
 
 def combine_tokens(y, position, weights, tokens, top_k):
-    """Inverse of permute_tokens for top-k routing: out[t] = sum_j weights[t, j] * y[position[t*k + j]]."""
+    """Inverse of permute_tokens for top-k routing: out[t] = sum_j weights[t, j] * y[position[t*k + j]].  Forward only, like
+    permute_tokens."""
     return weighted_sum_rows(y, position, weights, tokens, top_k)
 
 

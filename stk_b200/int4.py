@@ -193,9 +193,10 @@ def expert_mlp_int4(x, expert_ids, weights, w1, w2):
     """The experts' MLP of a dMoE layer on few tokens (decoding), from 4-bit weights:
     out[t] = sum_j weights[t, j] * W2_e GeLU(W1_e x[t]), e = expert_ids[t, j], [T, h_out] in x's type.
 
-    x [T, h] float16 or bfloat16; expert_ids [T, k] and weights [T, k] as top_k_gate gives them (a negative id
+    x [T, h] float16 or bfloat16 (forward only: a gradient or a tangent is refused); expert_ids [T, k] and weights [T, k] as top_k_gate gives them (a negative id
     contributes nothing); w1, w2: Int4Experts with f outputs and f inputs.  The hidden activations are rounded to x's
-    type, as in dmoe.expert_mlp; the sums over inputs and over choices are in 32 bits and rounded once."""
+    type, as in dmoe.expert_mlp (a tenth more error in the result at most); the sums over inputs and over choices are in 32
+    bits and rounded once."""
     _check_call("expert_mlp_int4", x, w1, expert_ids)
     refuse_tangents("expert_mlp_int4", weights)
     if not isinstance(w2, Int4Experts) or w2.num_experts != w1.num_experts or w2.inputs != w1.outputs \

@@ -209,7 +209,8 @@ def plan_tokens(expert_ids, num_experts, block=BLOCK, rows=None):
     """TokenPlan of expert_ids ([T] or [T, k], integers; a negative id: no expert): every expert's slots in order, its
     bin padded to a multiple of `block` rows.
 
-    rows None: as many rows as this batch needs - the one read-back of the step (the call waits for the stream).
+    rows None: as many rows as this batch needs, none for a batch without a live token - the one read-back of the step (the
+    call waits for the stream).
     rows = plan_rows(slots, num_experts) or more, a multiple of `block`: that many, the surplus as padding at the end
     of the last expert's bin; nothing waits for the device, and the step can be captured in a CUDA graph."""
     if expert_ids.dim() not in (1, 2) or expert_ids.dtype not in (torch.int16, torch.int32, torch.int64):
